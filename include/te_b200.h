@@ -389,6 +389,108 @@ TE_API int te_b200_cross_entropy(te_b200_ctx* ctx, const float* logits, const in
                           float* loss, float* dlogits, float upstream, int64_t rows, int64_t vocab,
                           te_stream_t stream);
 
+/* ---- answering token by token: rotary positions, key-value cache, attention over it ---- */
+/* No counterpart in the reference, whose attention always sees a whole sequence and whose positions are a fixed table
+ * added to the embedding (src/nn/positional_embedding.cpp:18-36).  Activations are FP32 like everywhere in this library
+ * and results are FP32-accurate; what varies is the type the cache keeps.  These entries check their descriptor before
+ * they look at the context, use no host synchronisation and may be captured into a CUDA graph. */
+
+/* Frequencies of rotary positions for a rotated width `rot` (even): out[j], j < rot/2, is the angle in radians by which
+ * pair j turns from one position to the next, base^(-2j/rot), changed for contexts longer than the trained one by
+ *   TE_ROTARY_LINEAR   every frequency divided by `factor`;
+ *   TE_ROTARY_BASE     the base multiplied by factor^(rot/(rot-2)): the slowest pair is stretched by `factor`, the fastest not;
+ *   TE_ROTARY_PARTS    pairs that make at most `slow_turns` turns over `trained_length` positions divided by `factor`, those
+ *                      that make at least `fast_turns` kept, linear in the number of turns between.
+ * Pure host arithmetic into host memory; needs no GPU and no context. */
+enum { TE_ROTARY_PLAIN = 0, TE_ROTARY_LINEAR = 1, TE_ROTARY_BASE = 2, TE_ROTARY_PARTS = 3 };
+TE_API int te_b200_rotary_inv_freq(int64_t rot, double base, int scaling, double factor, int64_t trained_length,
+                            double slow_turns, double fast_turns, double* out);
+
+/* y = x with the first `rot` elements of every head turned by its token's position:
+ *     (y0, y1) = scale * (x0 cos a - x1 sin a, x0 sin a + x1 cos a),   a = position * inv_freq[j],
+ * over the pairs (j, j + rot/2) or, with interleaved != 0, (2j, 2j + 1); elements from `rot` on are copied.
+ * inverse != 0 turns by -a: with the upstream gradient as x this is the backward pass (the transpose of the above).
+ * x and y are [B,H,T,d] views with element strides for B, H, T and unit stride over d, as te_attn_desc takes them: q and k
+ * head views of a projections' buffer need no copy, and adjacent q and k blocks are one view of 2H heads.  y may be x
+ * (same strides); otherwise the two must not overlap.  positions [B,T] (a stride of 0 shares one row) may be any int64
+ * below 2^40 in magnitude; angles are reduced in 64 bits.  d <= 1024. */
+typedef struct te_rotary_desc {
+    int64_t B, H, T, d, rot;
+    const float* x; int64_t x_strides[3];
+    float* y;       int64_t y_strides[3];
+    const int64_t* positions; int64_t position_strides[2];
+    const double* inv_freq;      /* device, rot/2 */
+    float   scale;               /* multiplies the rotated elements; 1 unless the context is stretched */
+    int32_t interleaved;
+    int32_t inverse;
+    int32_t reserved;
+} te_rotary_desc;
+TE_API int te_b200_rotary(te_b200_ctx* ctx, const te_rotary_desc* d, te_stream_t stream);
+
+/* A paged cache of keys and values.  Position p of a sequence lives in slot p % page_size of the page that the
+ * sequence's row of the page table names at p / page_size.  Element i of (page, slot, head) is at
+ * page * strides[0] + head * strides[1] + slot * strides[2] + i of k resp. v, so any order of pages, heads and slots
+ * will do ([pages, heads, page_size, d] reads fastest).  d is a multiple of 16 and at most 256, the bases are 16-byte
+ * aligned and the strides multiples of 16 bytes.
+ * TE_KV_E4M3 keeps 8-bit floats (4 exponent and 3 mantissa bits, no infinity) and, for every (page, head, slot), a
+ * power of two that the row is measured in: the smallest 2^e (e >= -126) with max |x| <= 448 * 2^e, so a value is
+ * rounded once, to nearest even, and dividing by the scale rounds nothing.  Values that are not finite are kept as NaN
+ * and do not count towards the scale. */
+enum { TE_KV_F32 = 0, TE_KV_BF16 = 1, TE_KV_E4M3 = 2 };
+typedef struct te_kv_cache {
+    int64_t pages, heads, page_size, d;
+    void* k; int64_t k_strides[3];       /* elements: page, head, slot */
+    void* v; int64_t v_strides[3];
+    float* k_scale;                      /* TE_KV_E4M3 only, else NULL */
+    float* v_scale;
+    int64_t scale_strides[3];            /* of both: page, head, slot */
+    int32_t dtype;                       /* TE_KV_* */
+    int32_t reserved;
+} te_kv_cache;
+
+/* Moves tokens into (append) or out of (read) the cache.  k, v: [B,H,T,d] float views, unit stride over d, H the cache's
+ * heads.  positions [B,T]: where in its sequence each token stands; a negative one is padding, which append skips and read
+ * fills with zeros.  page_table: row b starts at b * page_table_stride and holds max_pages page numbers.
+ * A position beyond the table, or a page outside [0, pages), is skipped (read: zeros) and reported by
+ * te_b200_check_device_status.  Two tokens of one append must not name the same place (its content is unspecified then).
+ * Read takes NULL for k or v to leave it out. */
+typedef struct te_kv_desc {
+    te_kv_cache cache;
+    int64_t B, T;
+    float* k; int64_t k_strides[3];      /* B, H, T; read by append, written by read */
+    float* v; int64_t v_strides[3];
+    const int64_t* page_table; int64_t page_table_stride; int64_t max_pages;
+    const int64_t* positions;  int64_t position_strides[2];
+} te_kv_desc;
+TE_API int te_b200_kv_append(te_b200_ctx* ctx, const te_kv_desc* d, te_stream_t stream);
+TE_API int te_b200_kv_read(te_b200_ctx* ctx, const te_kv_desc* d, te_stream_t stream);
+
+/* Attention of one new token per row over the row's cached tokens: with n = lens[r] and head h reading the keys and
+ * values of cache head h / (q_heads / heads),
+ *     o[r,h] = sum_t softmax_t(scale * q[r,h] . k[t]) v[t],   t in [max(0, n - window), n)   (window 0: from 0).
+ * q_heads is a multiple of the cache's heads.  lse (optional, [rows, q_heads] dense) receives
+ * log sum_t exp(scale * q.k[t]), with which results over parts of a sequence can be joined.  A row with lens[r] <= 0 gives
+ * zeros and -infinity.  Cached tokens outside the range are never read.  Rows may share pages, or whole rows of the table
+ * (page_table_stride 0): several tokens of one sequence are rows with growing lens.  lens beyond
+ * max_pages * page_size is cut to it, and a page outside [0, pages) counts as masked; both are reported by
+ * te_b200_check_device_status.  Softmax statistics and sums are kept in FP32 and joined in a fixed order.
+ * Uses the context workspace. */
+typedef struct te_paged_attn_desc {
+    te_kv_cache cache;
+    int64_t rows, q_heads;
+    const float* q; int64_t q_strides[2];   /* row, head; unit stride over d */
+    float* o;       int64_t o_strides[2];
+    float* lse;
+    const int64_t* page_table; int64_t page_table_stride; int64_t max_pages;
+    const int64_t* lens;                    /* [rows] */
+    int64_t window;
+    float   scale;                          /* usually 1 / sqrt(d) */
+    int32_t reserved;
+} te_paged_attn_desc;
+TE_API int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* d, te_stream_t stream);
+/* Workspace bytes the call above needs on a GPU with `sm_count` SMs; checks the descriptor.  Pure host arithmetic. */
+TE_API int te_b200_paged_attention_workspace_size(const te_paged_attn_desc* d, int sm_count, size_t* out_bytes);
+
 /* ---- introspection --------------------------------------------------------- */
 
 /* Which kernel form te_b200_gemm_f32 would use for this problem on a GPU with `sm_count` SMs

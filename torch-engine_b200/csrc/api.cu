@@ -26,9 +26,20 @@ int cuda_fail(cudaError_t e, const char* what) {
     return TE_ERR_CUDA;
 }
 
-static int fail(int code, const std::string& msg) {
+int fail(int code, const std::string& msg) {
     g_last_error = msg;
     return code;
+}
+
+int check_ctx(const te_b200_ctx* ctx) {
+    if (!ctx) return fail(TE_ERR_BAD_ARGUMENT, "ctx is NULL");
+    int cur = -1;
+    if (cudaGetDevice(&cur) != cudaSuccess || cur != ctx->device) {
+        char msg[128];
+        snprintf(msg, sizeof msg, "the context was created for device %d but device %d is current", ctx->device, cur);
+        return fail(TE_ERR_BAD_ARGUMENT, msg);
+    }
+    return TE_OK;
 }
 
 static inline int64_t round_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
@@ -191,19 +202,6 @@ static int gemm_device(te_b200_ctx* ctx, const te_gemm_desc* d, cudaStream_t st,
 
 using namespace te;
 
-// Every compute entry launches on the caller's stream, which belongs to the context's device: that device has to be
-// the calling thread's current one (as it is for the reference, which only ever uses device 0).
-static int check_ctx(const te_b200_ctx* ctx) {
-    if (!ctx) return fail(TE_ERR_BAD_ARGUMENT, "ctx is NULL");
-    int cur = -1;
-    if (cudaGetDevice(&cur) != cudaSuccess || cur != ctx->device) {
-        char msg[128];
-        snprintf(msg, sizeof msg, "the context was created for device %d but device %d is current", ctx->device, cur);
-        return fail(TE_ERR_BAD_ARGUMENT, msg);
-    }
-    return TE_OK;
-}
-
 extern "C" {
 
 const char* te_b200_status_string(int status) {
@@ -299,6 +297,7 @@ int te_b200_check_device_status(te_b200_ctx* ctx) {
         cudaMemset(ctx->d_status, 0, sizeof(int));
         if (h == STATUS_BAD_EMBEDDING_INDEX) return fail(TE_ERR_BAD_ARGUMENT, "Embedding index out of range");   // src/nn/embedding.cpp:53-55
         if (h == STATUS_BAD_TARGET_INDEX) return fail(TE_ERR_BAD_ARGUMENT, "Cross-entropy target index out of range");
+        if (h == STATUS_BAD_CACHE_PLACE) return fail(TE_ERR_BAD_ARGUMENT, "KV cache: position beyond the page table or page number out of range");
         char msg[128];
         snprintf(msg, sizeof msg, "device-side bounded wait gave up (site code %d)", h);
         return fail(TE_ERR_DEVICE_TIMEOUT, msg);

@@ -1,0 +1,196 @@
+// Rotary positions: pairs of a head's elements turned by angle position * inv_freq[pair], forward and (turned back) backward.
+//
+//     (y0, y1) = scale * (x0 cos a - x1 sin a, x0 sin a + x1 cos a)
+//
+// Bound by HBM: 4 B read and 4 B written per element.  The angle is the same for every head of a token, so a thread keeps
+// the cosines and sines of its pairs in registers and walks the heads with them; nothing goes through shared memory and no
+// thread waits for another.  Angles: position * inv_freq is formed and reduced to a fraction of a turn in FP64 (an FP32
+// product is off by 2^-24 of the whole angle, 0.06 rad at position 10^6); the fraction, below one half, goes to
+// sincospif in FP32.
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "pdl.cuh"
+#include "te_internal.h"
+
+namespace te {
+
+namespace {
+
+struct RotaryParams {
+    const float* x;
+    float* y;
+    const long long* positions;
+    const double* inv_freq;
+    long long xs[3], ys[3], ps[2];
+    long long total;             // threads with work: tokens * head_lanes * items
+    int T, H, rot, d;
+    int head_lanes;              // threads that share the heads of a (token, item)
+    int rot_items, items;        // of a head: groups of pairs, then groups of copied elements
+    float scale, sign;
+};
+
+// W pairs (or W copied elements) a thread: W = 4 moves float4s and needs rot and d in multiples of 8 and 4, aligned views.
+template <int W, bool INTERLEAVED>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
+    griddep_wait();
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= p.total) return;
+    long long rest = i / p.items;
+    const int item = (int)(i - rest * p.items);
+    const long long token = rest / p.head_lanes;
+    const int lane = (int)(rest - token * p.head_lanes);
+    const long long b = token / p.T;
+    const int t = (int)(token - b * p.T);
+    const float* x = p.x + b * p.xs[0] + t * p.xs[2];
+    float* y = p.y + b * p.ys[0] + t * p.ys[2];
+    if (item >= p.rot_items) {      // behind the rotated part
+        const int c = p.rot + (item - p.rot_items) * W;
+        for (int h = lane; h < p.H; h += p.head_lanes) {
+            if constexpr (W == 4) *reinterpret_cast<float4*>(y + h * p.ys[1] + c) = *reinterpret_cast<const float4*>(x + h * p.xs[1] + c);
+            else y[h * p.ys[1] + c] = x[h * p.xs[1] + c];
+        }
+        return;
+    }
+    const int j = item * W;         // first pair
+    const double position = (double)p.positions[b * p.ps[0] + t * p.ps[1]];
+    float c[W], s[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const double turns = position * p.inv_freq[j + w] * 0.15915494309189535;      // 1 / (2 pi)
+        const float part = (float)(turns - rint(turns));
+        sincospif(2.0f * part, &s[w], &c[w]);
+        c[w] *= p.scale;
+        s[w] *= p.scale * p.sign;
+    }
+    // element offsets of the thread's two vectors; interleaved pairs lie side by side in them
+    const int o0 = INTERLEAVED ? 2 * j : j, o1 = INTERLEAVED ? 2 * j + W : j + p.rot / 2;
+#pragma unroll 2
+    for (int h = lane; h < p.H; h += p.head_lanes) {
+        const float* xh = x + h * p.xs[1];
+        float* yh = y + h * p.ys[1];
+        float a[W], e[W];
+        if constexpr (W == 4) {
+            const float4 u = *reinterpret_cast<const float4*>(xh + o0), v = *reinterpret_cast<const float4*>(xh + o1);
+            a[0] = u.x; a[1] = u.y; a[2] = u.z; a[3] = u.w;
+            e[0] = v.x; e[1] = v.y; e[2] = v.z; e[3] = v.w;
+        } else {
+            a[0] = xh[o0];
+            e[0] = xh[o1];
+        }
+        if constexpr (INTERLEAVED && W == 4) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const float u0 = a[2 * w], u1 = a[2 * w + 1], v0 = e[2 * w], v1 = e[2 * w + 1];
+                a[2 * w] = u0 * c[w] - u1 * s[w];
+                a[2 * w + 1] = u0 * s[w] + u1 * c[w];
+                e[2 * w] = v0 * c[w + 2] - v1 * s[w + 2];
+                e[2 * w + 1] = v0 * s[w + 2] + v1 * c[w + 2];
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float u = a[w], v = e[w];
+                a[w] = u * c[w] - v * s[w];
+                e[w] = u * s[w] + v * c[w];
+            }
+        }
+        if constexpr (W == 4) {
+            *reinterpret_cast<float4*>(yh + o0) = make_float4(a[0], a[1], a[2], a[3]);
+            *reinterpret_cast<float4*>(yh + o1) = make_float4(e[0], e[1], e[2], e[3]);
+        } else {
+            yh[o0] = a[0];
+            yh[o1] = e[0];
+        }
+    }
+}
+
+bool vector_view(const float* p, const int64_t s[3]) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ((s[0] | s[1] | s[2]) & 3) == 0;
+}
+
+}  // namespace
+
+}  // namespace te
+
+using namespace te;
+
+extern "C" {
+
+int te_b200_rotary_inv_freq(int64_t rot, double base, int scaling, double factor, int64_t trained_length, double slow_turns,
+                            double fast_turns, double* out) {
+    if (rot < 0 || (rot & 1)) return fail(TE_ERR_BAD_ARGUMENT, "rotary: the rotated width must be even and not negative");
+    if (!(base > 0.0)) return fail(TE_ERR_BAD_ARGUMENT, "rotary: base must be positive");
+    if (scaling < TE_ROTARY_PLAIN || scaling > TE_ROTARY_PARTS) return fail(TE_ERR_BAD_ARGUMENT, "rotary: scaling must be a TE_ROTARY_* value");
+    if (scaling != TE_ROTARY_PLAIN && !(factor > 0.0)) return fail(TE_ERR_BAD_ARGUMENT, "rotary: factor must be positive");
+    if (scaling == TE_ROTARY_BASE && rot <= 2) return fail(TE_ERR_BAD_ARGUMENT, "rotary: TE_ROTARY_BASE needs more than one pair");
+    if (scaling == TE_ROTARY_PARTS && (trained_length < 1 || !(fast_turns > slow_turns)))
+        return fail(TE_ERR_BAD_ARGUMENT, "rotary: TE_ROTARY_PARTS needs trained_length >= 1 and fast_turns > slow_turns");
+    if (rot > 0 && !out) return fail(TE_ERR_BAD_ARGUMENT, "rotary: NULL pointer");
+    if (scaling == TE_ROTARY_BASE) base *= pow(factor, (double)rot / (double)(rot - 2));
+    for (int64_t j = 0; j < rot / 2; ++j) {
+        double f = pow(base, -2.0 * (double)j / (double)rot);
+        if (scaling == TE_ROTARY_LINEAR) {
+            f /= factor;
+        } else if (scaling == TE_ROTARY_PARTS) {
+            const double turns = (double)trained_length * f / 6.283185307179586;
+            double keep = (turns - slow_turns) / (fast_turns - slow_turns);
+            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
+            f *= keep + (1.0 - keep) / factor;
+        }
+        out[j] = f;
+    }
+    return TE_OK;
+}
+
+int te_b200_rotary(te_b200_ctx* ctx, const te_rotary_desc* t, te_stream_t stream) {
+    if (!t || t->B < 0 || t->H < 0 || t->T < 0 || t->d < 0) return fail(TE_ERR_BAD_ARGUMENT, "rotary: bad extents");
+    if (t->rot < 0 || (t->rot & 1) || t->rot > t->d) return fail(TE_ERR_BAD_ARGUMENT, "rotary: the rotated width must be even and at most d");
+    if (t->d > 1024) return fail(TE_ERR_BAD_ARGUMENT, "rotary: heads longer than 1024 elements are not supported");
+    if (t->H > INT32_MAX || t->T > INT32_MAX || (t->T > 0 && t->B > INT32_MAX / t->T)) return fail(TE_ERR_BAD_ARGUMENT, "rotary: extent exceeds 2^31-1");
+    if (t->B > 0 && t->H > 0 && t->T > 0 && t->d > 0) {
+        if (!t->x || !t->y || (t->rot > 0 && (!t->positions || !t->inv_freq))) return fail(TE_ERR_BAD_ARGUMENT, "rotary: NULL pointer");
+        const int64_t ext[3] = {t->B, t->H, t->T};
+        for (int i = 0; i < 3; ++i) {
+            if (t->x_strides[i] < 0 || t->y_strides[i] < 0) return fail(TE_ERR_BAD_ARGUMENT, "rotary: negative stride");
+            if (ext[i] > 1 && t->y_strides[i] < t->d) return fail(TE_ERR_UNSUPPORTED_LAYOUT, "rotary: heads of the output overlap");
+            if (t->x == t->y && ext[i] > 1 && t->x_strides[i] != t->y_strides[i])
+                return fail(TE_ERR_UNSUPPORTED_LAYOUT, "rotary: in place needs equal strides of input and output");
+        }
+        if (t->position_strides[0] < 0 || t->position_strides[1] < 0) return fail(TE_ERR_BAD_ARGUMENT, "rotary: negative stride");
+    }
+    if (int bad = check_ctx(ctx)) return bad;
+    if (t->B == 0 || t->H == 0 || t->T == 0 || t->d == 0) return TE_OK;
+    RotaryParams p;
+    p.x = t->x; p.y = t->y;
+    p.positions = reinterpret_cast<const long long*>(t->positions);
+    p.inv_freq = t->inv_freq;
+    for (int i = 0; i < 3; ++i) { p.xs[i] = t->x_strides[i]; p.ys[i] = t->y_strides[i]; }
+    p.ps[0] = t->position_strides[0]; p.ps[1] = t->position_strides[1];
+    p.T = (int)t->T; p.H = (int)t->H; p.rot = (int)t->rot; p.d = (int)t->d;
+    p.scale = t->scale;
+    p.sign = t->inverse ? -1.0f : 1.0f;
+    const bool vec = vector_view(t->x, t->x_strides) && vector_view(t->y, t->y_strides) && p.rot % 8 == 0 && p.d % 4 == 0;
+    const int w = vec ? 4 : 1;
+    p.rot_items = p.rot / (2 * w);
+    p.items = p.rot_items + (t->x == t->y ? 0 : (p.d - p.rot) / w);
+    if (p.items == 0) return TE_OK;                  // in place with nothing to turn
+    // One thread per (token, item) when that fills the GPU; otherwise its heads are shared among several.
+    const long long base = t->B * t->T * p.items, fill = (long long)ctx->sm_count * 2048;
+    long long lanes = (fill + base - 1) / base;
+    p.head_lanes = (int)(lanes > p.H ? p.H : lanes);
+    p.total = base * p.head_lanes;
+    const long long blocks = (p.total + 255) / 256;
+    if (blocks > INT32_MAX) return fail(TE_ERR_BAD_ARGUMENT, "rotary: too many elements");
+    const dim3 grid((unsigned)blocks), block(256);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (vec) e = t->interleaved ? launch_pdl(rotary_kernel<4, true>, grid, block, 0, st, p) : launch_pdl(rotary_kernel<4, false>, grid, block, 0, st, p);
+    else e = t->interleaved ? launch_pdl(rotary_kernel<1, true>, grid, block, 0, st, p) : launch_pdl(rotary_kernel<1, false>, grid, block, 0, st, p);
+    if (e != cudaSuccess) return cuda_fail(e, "rotary_kernel launch");
+    ctx->launches += 1;
+    return TE_OK;
+}
+
+}  // extern "C"

@@ -78,6 +78,11 @@ struct te_b200_ctx {
 namespace te {
 
 void set_error(const std::string& msg);
+// set_error, returning the code.
+int fail(int code, const std::string& msg);
+// Every compute entry launches on the caller's stream, which belongs to the context's device: that device has to be
+// the calling thread's current one (as it is for the reference, which only ever uses device 0).
+int check_ctx(const te_b200_ctx* ctx);
 int cuda_fail(cudaError_t e, const char* what);
 
 // cuTensorMapEncodeTiled for a 4-D fp32 tensor through the context's cache.  Returns the driver's CUresult (0 = ok).
@@ -91,6 +96,7 @@ constexpr int STATUS_COUNTER_WORDS = STATUS_AREA_BYTES / 4 - STATUS_COUNTER_WORD
 // Device status codes that are not wait sites.
 constexpr int STATUS_BAD_EMBEDDING_INDEX = 201;   // "Embedding index out of range" (src/nn/embedding.cpp:53-55)
 constexpr int STATUS_BAD_TARGET_INDEX = 202;      // cross-entropy target outside [0, vocab)
+constexpr int STATUS_BAD_CACHE_PLACE = 203;       // a position beyond the page table, or a page outside the cache
 constexpr int STATUS_SELFTEST_WAIT = 901;         // the wait self-test's barrier, which nobody arrives at
 
 // True when TMA can address the operand in place (16-byte aligned base, strides multiple of 16 B).
@@ -163,5 +169,8 @@ int launch_embedding_backward(te_b200_ctx*, const int64_t* tokens, const float* 
                               int64_t vocab, cudaStream_t);
 int launch_cross_entropy(te_b200_ctx*, const float* logits, const int64_t* targets, float* loss, float* grad, float upstream,
                          int64_t rows, int64_t V, cudaStream_t);
+
+// rotary.cu, kv_cache.cu, paged_attention.cu: rotary positions, the paged key-value cache and the attention over it
+int check_kv_cache(const te_kv_cache& c, const char* who);    // kv_cache.cu: the descriptor on its own
 
 }  // namespace te

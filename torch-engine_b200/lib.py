@@ -15,6 +15,8 @@ TE_ROW_MAJOR, TE_COL_MAJOR = 0, 1
 TE_PREC_TF32, TE_PREC_3XTF32 = 0, 1
 TE_EPI_NONE, TE_EPI_BIAS, TE_EPI_BIAS_GELU = 0, 1, 2
 TE_SCALE_NONE, TE_SCALE_MUL, TE_SCALE_DIV = 0, 1, 2
+TE_ROTARY_PLAIN, TE_ROTARY_LINEAR, TE_ROTARY_BASE, TE_ROTARY_PARTS = 0, 1, 2, 3
+TE_KV_F32, TE_KV_BF16, TE_KV_E4M3 = 0, 1, 2
 TE_B200_STATIC_SCRATCH_BYTES = 64 << 20
 
 c_float_p = C.POINTER(C.c_float)
@@ -80,6 +82,46 @@ class MhaBwdDesc(C.Structure):
                                                       ("wqkv", C.c_void_p), ("dwqkv", C.c_void_p), ("ld_qkv", C.c_int64)]
 
 
+class RotaryDesc(C.Structure):
+    """struct te_rotary_desc"""
+    _fields_ = [
+        ("B", C.c_int64), ("H", C.c_int64), ("T", C.c_int64), ("d", C.c_int64), ("rot", C.c_int64),
+        ("x", C.c_void_p), ("x_strides", C.c_int64 * 3), ("y", C.c_void_p), ("y_strides", C.c_int64 * 3),
+        ("positions", C.c_void_p), ("position_strides", C.c_int64 * 2), ("inv_freq", C.c_void_p),
+        ("scale", C.c_float), ("interleaved", C.c_int32), ("inverse", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class KvCacheDesc(C.Structure):
+    """struct te_kv_cache"""
+    _fields_ = [
+        ("pages", C.c_int64), ("heads", C.c_int64), ("page_size", C.c_int64), ("d", C.c_int64),
+        ("k", C.c_void_p), ("k_strides", C.c_int64 * 3), ("v", C.c_void_p), ("v_strides", C.c_int64 * 3),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("scale_strides", C.c_int64 * 3),
+        ("dtype", C.c_int32), ("reserved", C.c_int32),
+    ]
+
+
+class KvDesc(C.Structure):
+    """struct te_kv_desc"""
+    _fields_ = [
+        ("cache", KvCacheDesc), ("B", C.c_int64), ("T", C.c_int64),
+        ("k", C.c_void_p), ("k_strides", C.c_int64 * 3), ("v", C.c_void_p), ("v_strides", C.c_int64 * 3),
+        ("page_table", C.c_void_p), ("page_table_stride", C.c_int64), ("max_pages", C.c_int64),
+        ("positions", C.c_void_p), ("position_strides", C.c_int64 * 2),
+    ]
+
+
+class PagedAttnDesc(C.Structure):
+    """struct te_paged_attn_desc"""
+    _fields_ = [
+        ("cache", KvCacheDesc), ("rows", C.c_int64), ("q_heads", C.c_int64),
+        ("q", C.c_void_p), ("q_strides", C.c_int64 * 2), ("o", C.c_void_p), ("o_strides", C.c_int64 * 2), ("lse", C.c_void_p),
+        ("page_table", C.c_void_p), ("page_table_stride", C.c_int64), ("max_pages", C.c_int64), ("lens", C.c_void_p),
+        ("window", C.c_int64), ("scale", C.c_float), ("reserved", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/te_b200.h declares
 SIGNATURES = {
     "te_b200_init": (C.c_int, [C.c_int, C.c_size_t, C.POINTER(C.c_void_p)]),
@@ -120,6 +162,13 @@ SIGNATURES = {
     "te_b200_embedding_forward": (C.c_int, [C.c_void_p] + [C.c_void_p] * 4 + [C.c_int64] * 4 + [C.c_void_p]),
     "te_b200_embedding_backward": (C.c_int, [C.c_void_p] + [C.c_void_p] * 3 + [C.c_int64] * 3 + [C.c_void_p]),
     "te_b200_cross_entropy": (C.c_int, [C.c_void_p] + [C.c_void_p] * 4 + [C.c_float, C.c_int64, C.c_int64, C.c_void_p]),
+    "te_b200_rotary_inv_freq": (C.c_int, [C.c_int64, C.c_double, C.c_int, C.c_double, C.c_int64, C.c_double, C.c_double,
+                                          C.POINTER(C.c_double)]),
+    "te_b200_rotary": (C.c_int, [C.c_void_p, C.POINTER(RotaryDesc), C.c_void_p]),
+    "te_b200_kv_append": (C.c_int, [C.c_void_p, C.POINTER(KvDesc), C.c_void_p]),
+    "te_b200_kv_read": (C.c_int, [C.c_void_p, C.POINTER(KvDesc), C.c_void_p]),
+    "te_b200_paged_attention": (C.c_int, [C.c_void_p, C.POINTER(PagedAttnDesc), C.c_void_p]),
+    "te_b200_paged_attention_workspace_size": (C.c_int, [C.POINTER(PagedAttnDesc), C.c_int, C.POINTER(C.c_size_t)]),
     "te_b200_comm_unique_id": (C.c_int, [C.c_void_p]),
     "te_b200_comm_init": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),
     "te_b200_comm_destroy": (C.c_int, [C.c_void_p]),
@@ -178,6 +227,13 @@ def shard_range(total, world, rank, align=1):
     b, n = C.c_int64(), C.c_int64()
     check(load().te_b200_shard_range(total, world, rank, align, C.byref(b), C.byref(n)))
     return b.value, n.value
+
+
+def rotary_inv_freq(rot, base=10000.0, scaling=TE_ROTARY_PLAIN, factor=1.0, trained_length=0, slow_turns=1.0, fast_turns=32.0):
+    """The rot/2 angles per position of te_b200_rotary_inv_freq as a list of floats; needs no GPU."""
+    out = (C.c_double * max(rot // 2, 1))()
+    check(load().te_b200_rotary_inv_freq(rot, base, scaling, factor, trained_length, slow_turns, fast_turns, out))
+    return list(out)[:rot // 2]
 
 
 def matmul_shape(a_shape, a_strides, b_shape, b_strides):

@@ -13,6 +13,8 @@ used only as device-memory holders (data_ptr, shape, stride) and for the current
     Backend.softmax / softmax_backward / gelu / gelu_backward / colsum: the kernels between the GEMMs.
     Backend.layernorm / layernorm_backward / embedding / embedding_backward / cross_entropy: the GPT step's kernels
         around the matmuls (src/nn/layernorm.cpp, src/nn/embedding.cpp, src/loss/CrossEntropyLoss.cpp).
+    Backend.rotary / rotary_backward / kv_cache / kv_append / kv_read / paged_attention: what a trained model needs to
+        answer token by token (no reference counterpart: its attention always sees a whole sequence).
 """
 import ctypes as C
 
@@ -35,9 +37,54 @@ def _ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
+_KV_DTYPES = {torch.float32: L.TE_KV_F32, torch.bfloat16: L.TE_KV_BF16, torch.float8_e4m3fn: L.TE_KV_E4M3}
+_KV_NAMES = {"f32": torch.float32, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}
+_ROTARY_SCALINGS = {None: L.TE_ROTARY_PLAIN, "linear": L.TE_ROTARY_LINEAR, "base": L.TE_ROTARY_BASE, "parts": L.TE_ROTARY_PARTS}
+
+
+def _strides(t, n):
+    return (C.c_int64 * n)(*t.stride()[:n])
+
+
 def _i64(seq):
     n = max(len(seq), 1)
     return (C.c_int64 * n)(*seq)
+
+
+class KvCache:
+    """Keys and values of earlier tokens in pages: k, v [pages, heads, page_size, d] tensors (float32, bfloat16 or
+    float8_e4m3fn; any strides with a unit last one), and for float8 their scales [pages, heads, page_size] (float32).
+    Backend.kv_cache allocates one."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        bad = lambda text: L.BackendError(L.TE_ERR_BAD_ARGUMENT, "KvCache: " + text)
+        if k.dtype not in _KV_DTYPES or v.dtype != k.dtype:
+            raise bad("k and v must both be float32, bfloat16 or float8_e4m3fn")
+        if k.dim() != 4 or v.shape != k.shape:
+            raise bad("k and v must be of one [pages, heads, page_size, d] shape")
+        eight_bit = k.dtype == torch.float8_e4m3fn
+        scales = (k_scale, v_scale) if eight_bit else ()
+        if not eight_bit and (k_scale is not None or v_scale is not None):
+            raise bad("only a float8 cache has scales")
+        for t in scales:
+            if t is None or t.dtype != torch.float32 or t.shape != k.shape[:3] or t.stride() != k_scale.stride():
+                raise bad("a float8 cache needs float32 scales [pages, heads, page_size] of equal strides")
+        for t in (k, v) + scales:
+            if not t.is_cuda or t.device != k.device:
+                raise bad("all tensors must be on one GPU")
+        for t in (k, v):
+            if t.stride(3) != 1:
+                raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, "KvCache: the last dimension must have unit stride")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.pages, self.heads, self.page_size, self.d = k.shape
+        c = L.KvCacheDesc()
+        c.pages, c.heads, c.page_size, c.d = k.shape
+        c.k, c.v = k.data_ptr(), v.data_ptr()
+        c.k_strides, c.v_strides = _strides(k, 3), _strides(v, 3)
+        if eight_bit:
+            c.k_scale, c.v_scale, c.scale_strides = k_scale.data_ptr(), v_scale.data_ptr(), _strides(k_scale, 3)
+        c.dtype = _KV_DTYPES[k.dtype]
+        self.desc = c
 
 
 class Backend:
@@ -362,6 +409,138 @@ class Backend:
         L.check(self._lib.te_b200_cross_entropy(self._ctx, _ptr(logits), _ptr(targets), _ptr(loss), _ptr(grad), upstream, rows,
                                                 vocab, self._stream()))
         return loss, grad
+
+    # ------------------------------------------------------------------ answering token by token
+    def _check_here(self, who, dtype, *ts):
+        for t in ts:
+            if t.dtype != dtype or t.device != self.torch_device:
+                raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "%s: expected %s tensors on %s" % (who, dtype, self.torch_device))
+
+    def rotary_inv_freq(self, rot, base=10000.0, scaling=None, factor=1.0, trained_length=0, slow_turns=1.0, fast_turns=32.0):
+        """Angle per position of each of the rot/2 pairs (float64, on the device): base^(-2j/rot), for contexts beyond the
+        trained length stretched by scaling = "linear", "base" or "parts" (te_b200_rotary_inv_freq).  Build it once."""
+        if scaling not in _ROTARY_SCALINGS:
+            raise ValueError("scaling must be None, 'linear', 'base' or 'parts'")
+        f = L.rotary_inv_freq(rot, base, _ROTARY_SCALINGS[scaling], factor, trained_length, slow_turns, fast_turns)
+        return torch.tensor(f, dtype=torch.float64, device=self.torch_device)
+
+    def rotary(self, x, positions, inv_freq, interleaved=False, scale=1.0, out=None):
+        """x [B,H,T,d] (any view with a unit last stride, such as the head views of a projections' buffer) with the first
+        2 * len(inv_freq) elements of every head turned by position * inv_freq: pairs (j, j + rot/2), or (2j, 2j + 1) if
+        interleaved; the rest is copied.  positions: int64 [B,T], or [T] for all of the batch.  scale multiplies the turned
+        elements.  Returns a contiguous tensor, or out (which may be x)."""
+        return self._rotary(x, positions, inv_freq, interleaved, scale, out, 0)
+
+    def rotary_backward(self, dy, positions, inv_freq, interleaved=False, scale=1.0, out=None):
+        """Gradient of x given that of rotary's result: the same turned back."""
+        return self._rotary(dy, positions, inv_freq, interleaved, scale, out, 1)
+
+    def _rotary(self, x, positions, inv_freq, interleaved, scale, out, inverse):
+        self._check_here("rotary", torch.float32, x)
+        self._check_here("rotary", torch.int64, positions)
+        self._check_here("rotary", torch.float64, inv_freq)
+        if x.dim() != 4:
+            raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "rotary expects a [B,H,T,d] view")
+        B, H, T, dim = x.shape
+        shared = positions.dim() == 1
+        if tuple(positions.shape) != ((T,) if shared else (B, T)) or inv_freq.dim() != 1:
+            raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "rotary expects positions [B,T] or [T] and one-dimensional frequencies")
+        if out is None:
+            out = torch.empty((B, H, T, dim), dtype=torch.float32, device=x.device)
+        else:
+            self._check_here("rotary", torch.float32, out)
+            if out.shape != x.shape:
+                raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "rotary: out must be shaped like x")
+        if dim > 1 and (x.stride(3) != 1 or out.stride(3) != 1):
+            raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, "rotary: the last dimension must have unit stride")
+        d = L.RotaryDesc()
+        d.B, d.H, d.T, d.d, d.rot = B, H, T, dim, 2 * inv_freq.numel()
+        d.x, d.x_strides, d.y, d.y_strides = x.data_ptr(), _strides(x, 3), out.data_ptr(), _strides(out, 3)
+        d.positions = positions.data_ptr()
+        d.position_strides = (C.c_int64 * 2)(0, positions.stride(0)) if shared else _strides(positions, 2)
+        d.inv_freq = (inv_freq if inv_freq.is_contiguous() else inv_freq.contiguous()).data_ptr()
+        d.scale, d.interleaved, d.inverse = scale, int(bool(interleaved)), inverse
+        L.check(self._lib.te_b200_rotary(self._ctx, C.byref(d), self._stream()))
+        return out
+
+    def kv_cache(self, pages, heads, page_size, d, dtype="f32"):
+        """An empty cache of `pages` pages of page_size tokens for `heads` key heads of d elements (a multiple of 16, at most
+        256); dtype "f32", "bf16" or "e4m3" (8 bits and a power of two per row)."""
+        if dtype not in _KV_NAMES:
+            raise ValueError("dtype must be 'f32', 'bf16' or 'e4m3'")
+        k, v = (torch.zeros((pages, heads, page_size, d), dtype=_KV_NAMES[dtype], device=self.torch_device) for _ in range(2))
+        scales = [torch.ones((pages, heads, page_size), device=self.torch_device) for _ in range(2)] if dtype == "e4m3" else (None, None)
+        return KvCache(k, v, *scales)
+
+    def _kv_desc(self, who, cache, page_table, positions):
+        self._check_here(who, torch.int64, page_table, positions)
+        self._check_here(who, cache.k.dtype, cache.k)
+        if page_table.dim() != 2 or positions.dim() != 2 or page_table.shape[0] != positions.shape[0]:
+            raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, who + " expects page_table [B, pages] and positions [B,T]")
+        if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+            raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, who + ": rows of the page table must be contiguous")
+        d = L.KvDesc()
+        d.cache = cache.desc
+        d.B, d.T = positions.shape
+        d.page_table, d.page_table_stride, d.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
+        d.positions, d.position_strides = positions.data_ptr(), _strides(positions, 2)
+        return d
+
+    def kv_append(self, cache, k, v, page_table, positions):
+        """Writes k, v [B,H,T,d] (views with a unit last stride) into the cache: token (b, t) at positions[b, t] of sequence b,
+        in the page that page_table[b, position // page_size] names.  Negative positions are padding.  The places must
+        be distinct; those beyond the table or the cache are skipped and reported by check_device_status."""
+        d = self._kv_desc("kv_append", cache, page_table, positions)
+        self._check_here("kv_append", torch.float32, k, v)
+        for t in (k, v):
+            if tuple(t.shape) != (d.B, cache.heads, d.T, cache.d):
+                raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "kv_append expects k and v [B, heads, T, d] as the cache and the positions have them")
+            if t.stride(3) != 1:
+                raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, "kv_append: the last dimension must have unit stride")
+        d.k, d.k_strides, d.v, d.v_strides = k.data_ptr(), _strides(k, 3), v.data_ptr(), _strides(v, 3)
+        L.check(self._lib.te_b200_kv_append(self._ctx, C.byref(d), self._stream()))
+
+    def kv_read(self, cache, page_table, positions):
+        """(k, v) float32 [B,H,T,d] of the tokens at these positions, addressed as kv_append does; zeros at negative ones."""
+        d = self._kv_desc("kv_read", cache, page_table, positions)
+        k, v = (torch.empty((d.B, cache.heads, d.T, cache.d), dtype=torch.float32, device=self.torch_device) for _ in range(2))
+        d.k, d.k_strides, d.v, d.v_strides = k.data_ptr(), _strides(k, 3), v.data_ptr(), _strides(v, 3)
+        L.check(self._lib.te_b200_kv_read(self._ctx, C.byref(d), self._stream()))
+        return k, v
+
+    def paged_attention(self, q, cache, page_table, lens, scale=None, window=0, want_lse=False, out=None):
+        """Attention of one new token per row: q [rows, q_heads, d] over the first lens[row] cached tokens of the row's
+        sequence (the last `window` of them if window > 0), query head h reading key head h // (q_heads // heads).
+        scale: 1 / sqrt(d) unless given.  Returns o [rows, q_heads, d] (out if given), with want_lse (o, log-sum-exp
+        [rows, q_heads]).  A row of length zero gives zeros (and -inf)."""
+        who = "paged_attention"
+        self._check_here(who, torch.float32, q)
+        self._check_here(who, torch.int64, page_table, lens)
+        self._check_here(who, cache.k.dtype, cache.k)
+        if q.dim() != 3 or q.shape[2] != cache.d:
+            raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "paged_attention expects q [rows, q_heads, d] with the cache's d")
+        rows, heads, dim = q.shape
+        if page_table.dim() != 2 or page_table.shape[0] != rows or tuple(lens.shape) != (rows,):
+            raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "paged_attention expects page_table [rows, pages] and lens [rows]")
+        if out is None:
+            out = torch.empty((rows, heads, dim), dtype=torch.float32, device=q.device)
+        else:
+            self._check_here(who, torch.float32, out)
+            if out.shape != q.shape:
+                raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "paged_attention: out must be shaped like q")
+        if q.stride(2) != 1 or out.stride(2) != 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1) or (rows > 1 and lens.stride(0) != 1):
+            raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, "paged_attention: last dimensions must have unit stride")
+        lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if want_lse else None
+        d = L.PagedAttnDesc()
+        d.cache = cache.desc
+        d.rows, d.q_heads = rows, heads
+        d.q, d.q_strides, d.o, d.o_strides = q.data_ptr(), _strides(q, 2), out.data_ptr(), _strides(out, 2)
+        d.lse = lse.data_ptr() if want_lse else None
+        d.page_table, d.page_table_stride, d.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
+        d.lens = lens.data_ptr()
+        d.window, d.scale = window, dim ** -0.5 if scale is None else scale
+        L.check(self._lib.te_b200_paged_attention(self._ctx, C.byref(d), self._stream()))
+        return (out, lse) if want_lse else out
 
     # ------------------------------------------------------------------ row / elementwise ops
     def softmax(self, x):
