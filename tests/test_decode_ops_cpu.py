@@ -228,3 +228,56 @@ def test_eight_bit_grid_of_the_reference():
     assert out.tolist() == [448.0, 1.0, 0.0625, 16.0, 20.0, -2.0 ** -9, 0.0, 2.0 ** -8]
     assert ref.e4m3_row(np.array([448.0 * (1 + 2.0 ** -20)]))[1] == 2.0
     assert ref.e4m3_row(np.array([0.0]))[1] == 2.0 ** -126
+
+
+def test_shares_of_paged_attention_on_the_host(tmp_path):
+    """Every tile of every segment belongs to exactly one worker, a segment's workers are those that the join adds up, and
+    no worker holds more than one part of either kind."""
+    src = tmp_path / "shares.cpp"
+    src.write_text(r"""
+#include <stdio.h>
+#include <algorithm>
+#include <map>
+#include <vector>
+#include "paged_plan.h"
+using namespace te;
+int main() {
+    long bad = 0;
+    uint64_t x = 88172645463325252ull;
+    auto rnd = [&](uint64_t n) { x ^= x << 13; x ^= x >> 7; x ^= x << 17; return x % n; };
+    for (int trial = 0; trial < 3000; ++trial) {
+        const int tile = trial % 2 ? 64 : 32, heads = 1 + (int)rnd(9), rows = 1 + (int)rnd(12), grid = 1 + (int)rnd(trial % 3 ? 300 : 7);
+        const int64_t window = rnd(3) ? 0 : 1 + (int64_t)rnd(500), most = 3000;
+        int64_t units = 0;
+        std::vector<int64_t> begin, end;            // of segments with tiles
+        for (int r = 0; r < rows; ++r) {
+            const int64_t len = (int64_t)rnd(8) == 0 ? -(int64_t)rnd(3) : (int64_t)rnd(trial % 5 ? 3500 : 70);
+            const RowRange range = row_range(len, most, window);
+            bad += range.n != std::max<int64_t>(0, std::min(len, most)) || range.first != (window ? std::max<int64_t>(0, range.n - window) : 0);
+            const int c = row_tiles(range, tile);
+            if (range.n > range.first) bad += c != (range.n - 1) / tile - range.first / tile + 1; else bad += c != 0;
+            for (int h = 0; h < heads && c; ++h) { begin.push_back(units); units += c; end.push_back(units); }
+        }
+        if (!units) continue;
+        const int workers = (int)std::min<int64_t>(grid, units);
+        bad += worker_begin(units, workers, 0) != 0 || worker_begin(units, workers, workers) != units;
+        for (int w = 0; w < workers; ++w) bad += worker_begin(units, workers, w + 1) <= worker_begin(units, workers, w);
+        for (int64_t u = 0; u < units; ++u) {
+            const int w = worker_of(units, workers, u);
+            bad += w < 0 || w >= workers || u < worker_begin(units, workers, w) || u >= worker_begin(units, workers, w + 1);
+        }
+        std::map<int, int> used;
+        for (size_t s = 0; s < begin.size(); ++s) {
+            const int first = worker_of(units, workers, begin[s]), last = worker_of(units, workers, end[s] - 1);
+            if (first == last) continue;
+            for (int w = first; w <= last; ++w) used[part_slot(w, w == first)]++;
+        }
+        for (auto& u : used) bad += u.second != 1 || u.first < 0 || u.first >= 2 * workers;
+    }
+    printf("%ld\n", bad);
+    return 0;
+}
+""")
+    exe = tmp_path / "shares"
+    subprocess.run(["g++", "-std=c++17", "-O2", "-I", os.path.join(ROOT, "torch-engine_b200", "csrc"), str(src), "-o", str(exe)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.strip() == "0"

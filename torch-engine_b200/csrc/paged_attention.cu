@@ -2,15 +2,28 @@
 //
 //     o = sum_t p_t v_t / sum_t p_t,   p_t = exp(scale * q . k_t - m),   m the running maximum
 //
-// One pass over the row's keys and values; the sums are rescaled when the maximum grows.  All arithmetic in FP32.
+// Bound by reading the cache once: 2 d values of 4, 2 or 1 byte per cached token and key head.  What follows from that:
+//
+// * Query heads that share a key head are computed together (up to 8, a head tile), so that a value is read once for all.
+// * A fixed number of thread blocks, all resident, share the tiles of all rows evenly (paged_plan.h), so that one long
+//   sequence, many short ones and any mixture keep every SM reading.  A block that holds only part of a (row, head tile)
+//   leaves its sums in the workspace; paged_join_kernel adds the parts in their order.
+// * Keys and values go from global memory straight into the registers that the arithmetic reads, 16 bytes a lane, the next
+//   tokens' loads in flight during the arithmetic of the current ones; nothing is staged in shared memory.
+//
+// 2- and 1-byte caches use the tensor cores through mma.sync m16n8k16 (8 query rows do not fill the 128-row tiles of
+// tcgen05, and the products need 5 % of the tensor rate): a stored value is exactly a bf16 resp. half, and an FP32 query
+// or weight is exactly (to 2^-24 of its row's largest) the sum of three bf16 resp. two half terms, so that products and
+// sums are those of FP32.  The terms of a head occupy rows g and g + 8 of one tile, both in the same thread.  Which element of a head
+// an index of the contraction stands for is free as long as both operands agree, and chosen so that a lane's 16 bytes are
+// its operand.  An FP32 cache uses FP32 FMAs (two per instruction).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
-#include "kv_place.h"
+#include "paged_plan.h"
 #include "pdl.cuh"
 #include "te_internal.h"
 
@@ -18,96 +31,908 @@ namespace te {
 
 namespace {
 
+constexpr int WARPS = 4;
+constexpr int THREADS = 32 * WARPS;
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
 struct AttnParams {
     const float* q;
     float* o;
     float* lse;
-    const void* kc;
-    const void* vc;
+    const char* kc;
+    const char* vc;
     const float* k_scale;
     const float* v_scale;
     const int64_t* page_table;
     const int64_t* lens;
-    int64_t qs[2], os[2], kcs[3], vcs[3], ss[3];
+    int64_t qs[2], os[2];
+    int64_t kcs[3], vcs[3];       // bytes
+    int64_t ss[3];                // elements
     int64_t table_stride, max_pages, pages, window;
-    int64_t rows;
     FastDivisor page_size;
-    int q_heads, group, d;
+    int rows, q_heads, kv_heads, group, head_tiles, d;
     float scale;
+    float* part_acc;              // [2 * workers][heads of a tile][d]
+    float2* part_ml;              // [2 * workers][heads of a tile]: running maximum (base 2) and sum
+    int4* joins;                  // [workers]: row, head tile, last worker, 1 -- of the segment that begins in this share and is split
     int* status;
 };
 
-template <int DTYPE>
-__device__ __forceinline__ float stored_value(const void* base, int64_t at) {
-    if constexpr (DTYPE == TE_KV_F32) return static_cast<const float*>(base)[at];
-    else if constexpr (DTYPE == TE_KV_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at]);
-    else return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const __nv_fp8_storage_t*>(base)[at], __NV_E4M3)));
-}
+struct Segment {
+    int row, kv_head, head0, heads;       // query heads head0 .. head0 + heads - 1
+    RowRange range;
+};
 
-// One warp per (row, query head), lanes along d.
-template <int DTYPE>
-__global__ void __launch_bounds__(32) paged_attention_kernel(const AttnParams p) {
-    griddep_wait();
-    const int lane = threadIdx.x;
-    const int64_t r = blockIdx.x / p.q_heads;
-    const int h = (int)(blockIdx.x - r * p.q_heads), kh = h / p.group;
-    int64_t n = p.lens[r];
-    const int64_t most = p.max_pages * (int64_t)p.page_size.divisor;
-    if (n > most) {
-        n = most;
-        if (lane == 0) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
+// ---------------------------------------------------------------------------------------------------- small pieces
+__device__ __forceinline__ void mma_bf16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ float bf16_lo(unsigned v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float bf16_hi(unsigned v) { return __uint_as_float(v & 0xffff0000u); }
+__device__ __forceinline__ unsigned pack_half(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned*>(&v);
+}
+__device__ __forceinline__ float2 unpack_half(unsigned v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+// Two e4m3 values (low byte first) as two halves, exactly.
+__device__ __forceinline__ unsigned half_of_e4m3(unsigned two) {
+    unsigned r;
+    asm("{ .reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t; }" : "=r"(r) : "r"(two));
+    return r;
+}
+__device__ __forceinline__ uint4 load16(const char* p, bool there) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (there) v = __ldg(reinterpret_cast<const uint4*>(p));
+    return v;
+}
+__device__ __forceinline__ unsigned long long pair(float x, float y) {
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ float2 unpair(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ void fma2(unsigned long long& d, unsigned long long a, unsigned long long b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// exp2 of a score less the maximum; a maximum of -infinity means that nothing has been seen.
+__device__ __forceinline__ float settled(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// The pages that hold N consecutive tokens from t0 (a multiple of N).  ALIGNED: one page holds them all.
+template <bool ALIGNED, int N>
+struct Places {
+    int64_t entry;     // as read, of token (lane & (N - 1)) resp. of all
+    int page;
+    unsigned slot;
+    __device__ __forceinline__ void fetch(const AttnParams& p, const int64_t* table, int64_t t0, int lane, int64_t n) {
+        const int64_t t = ALIGNED ? t0 : t0 + (lane & (N - 1));
+        entry = -1;
+        slot = 0;
+        if (t < n) {                       // n is within the table
+            const unsigned i = fast_quotient((unsigned)t, p.page_size);
+            slot = (unsigned)t - i * p.page_size.divisor;
+            entry = __ldg(table + i);
+        }
     }
-    const int64_t first = p.window > 0 && n > p.window ? n - p.window : 0;
-    const PageRow table = {p.page_table + r * p.table_stride, p.max_pages, p.pages};
-    float q[8], acc[8];
-    const int per = (p.d + 31) / 32;
+    // Checks what fetch read; reports a page outside the cache that a token of [first, n) lies in.
+    __device__ __forceinline__ void settle(const AttnParams& p, int64_t t0, int lane, const RowRange& range) {
+        const bool good = entry >= 0 && entry < p.pages;
+        page = good ? (int)entry : -1;
+        const int64_t t = ALIGNED ? t0 : t0 + (lane & (N - 1));
+        if (!good && t < range.n && (ALIGNED ? t + N > range.first : t >= range.first)) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
+    }
+    __device__ __forceinline__ int page_of(int i) const { return ALIGNED ? page : __shfl_sync(0xffffffffu, page, i); }
+    __device__ __forceinline__ unsigned slot_of(int i) const { return ALIGNED ? slot + i : __shfl_sync(0xffffffffu, slot, i); }
+};
+
+// ------------------------------------------------------------------------------------------- 2- and 1-byte caches
+// One warp's share of a segment on the tensor cores: 16 tokens at a time.
+//
+// Lane (g, r) = (lane / 4, lane % 4).  Scores S = Q K^T: the lane's operand of K is 16 bytes of tokens g and 8 + g; it receives the
+// scores of head g with tokens 2r, 2r + 1, 8 + 2r, 9 + 2r.  Values O = P V: weights of just these tokens are its operand of P, and its
+// operand of V is 16 (or 8) bytes of the same four tokens, two tokens' values interleaved by byte permutes.
+template <int DTYPE, int DP>
+struct TensorWarp {
+    static constexpr int HEADS = 8, TOKENS = 16;
+    static constexpr bool E4M3 = DTYPE == TE_KV_E4M3;
+    static constexpr int ES = E4M3 ? 1 : 2;
+    static constexpr int KG = E4M3 ? DP / 64 : DP / 32;                 // groups of 4 lanes x 16 bytes of a key
+    static constexpr int KB = KG > 4 ? 4 : KG;                          // of which this many are in registers at a time
+    static constexpr int VW = E4M3 && DP < 128 ? 8 : 16;                // bytes of a value a lane holds per chunk
+    static constexpr int VE = VW / ES;                                  // elements of it
+    static constexpr int VC = DP / (8 * VE);                            // chunks of 8 lanes
+    static constexpr int VB = VC > 2 ? 2 : VC;
+    static constexpr int QWORDS = E4M3 ? 16 : 12;                       // 32-bit words of query terms per (group, lane)
+    static constexpr int Q_BYTES = KG * 32 * QWORDS * 4;
+    static constexpr float LIFT = 10.0f;        // e4m3: weights reach 2^10, so that the lower of their two half terms keeps 2^-34 of the largest
+
+    // Splits the tile's queries into terms, in the order the tensor operand wants them.  q_unit: e4m3 only, what the scores of a head
+    // are measured in (the terms are the query brought to below 2^13 by a power of two).
+    static __device__ void stage_queries(const AttnParams& p, const Segment& s, unsigned* words, float* q_unit) {
+        const float* q = p.q + s.row * p.qs[0] + s.head0 * p.qs[1];
+        if constexpr (E4M3) {
+            const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+            for (int h = warp; h < HEADS; h += WARPS) {
+                float top = 0.0f;
+                if (h < s.heads)
+                    for (int c = lane; c < p.d; c += 32) top = fmaxf(top, fabsf(q[h * p.qs[1] + c]));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = lane + 32 * i;
-        q[i] = i < per && c < p.d ? p.q[r * p.qs[0] + h * p.qs[1] + c] * p.scale : 0.0f;
-        acc[i] = 0.0f;
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                int e = (int)(__float_as_uint(top) >> 23) - 126 - 13;          // top < 2^(e + 13)
+                e = e < -100 ? -100 : e > 100 ? 100 : e;
+                if (lane == 0) q_unit[h] = __uint_as_float((unsigned)(e + 127) << 23);
+            }
+            __syncthreads();
+        }
+        // one thread per (group, lane, pair of elements)
+        constexpr int PAIRS = E4M3 ? 8 : 4;
+        for (int i = threadIdx.x; i < KG * 32 * PAIRS; i += THREADS) {
+            const int j = i % PAIRS, lane = i / PAIRS % 32, c = i / PAIRS / 32;
+            const int g = lane / 4, r = lane % 4;
+            const int at = (E4M3 ? 64 * c + 16 * r : 32 * c + 8 * r) + 2 * j;
+            float x = 0.0f, y = 0.0f;
+            if (g < s.heads && at < p.d) {
+                x = q[g * p.qs[1] + at];
+                y = q[g * p.qs[1] + at + 1];
+            }
+            unsigned* w = words + (c * 32 + lane) * 4;                 // [term quarter][group][lane][4]
+            constexpr int QUARTER = KG * 32 * 4;
+            if constexpr (E4M3) {
+                const float unit = 1.0f / q_unit[g];                   // a power of two
+                x *= unit;
+                y *= unit;
+                const unsigned hi = pack_half(x, y);
+                const float2 f = unpack_half(hi);
+                w[(j / 4) * QUARTER + j % 4] = hi;
+                w[(2 + j / 4) * QUARTER + j % 4] = pack_half(x - f.x, y - f.y);
+            } else {
+                const unsigned hi = pack_bf16(x, y);
+                x -= bf16_lo(hi);
+                y -= bf16_hi(hi);
+                const unsigned mid = pack_bf16(x, y);
+                w[j] = hi;
+                w[QUARTER + j] = mid;
+                w[2 * QUARTER + j] = pack_bf16(x - bf16_lo(mid), y - bf16_hi(mid));
+            }
+        }
     }
-    float m = -INFINITY, l = 0.0f;
-    for (int64_t t = first; t < n; ++t) {
-        int64_t page;
-        uint32_t slot;
-        if (!kv_place(table, p.page_size, t, page, slot)) {
-            if (lane == 0) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
+
+    float acc[VC * VE][4];     // [n tile][row g: 2 columns, row g + 8: 2 columns]
+    float m, l;                // of head g; l over this lane's tokens only
+    float mv;                  // e4m3: the maximum the values' weights are measured against
+
+    template <bool ALIGNED>
+    __device__ void run(const AttnParams& p, const Segment& s, const unsigned* words, const float* q_unit, int64_t tile, int64_t tile_end) {
+        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, r = lane % 4;
+        const int64_t* table = p.page_table + s.row * p.table_stride;
+        const RowRange range = s.range;
+        constexpr int64_t STEP = WARPS * TOKENS;
+        int64_t t0 = tile * STEP + warp * TOKENS;
+        const int64_t t_end = tile_end * STEP;
+#pragma unroll
+        for (int i = 0; i < VC * VE; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+        m = mv = -INFINITY;
+        l = 0.0f;
+        const char* kbase = p.kc + s.kv_head * p.kcs[1] + r * 16;
+        const char* vbase = p.vc + s.kv_head * p.vcs[1] + g * VW;
+        const float unit = p.scale * LOG2E * (E4M3 ? q_unit[g] : 1.0f);
+        Places<ALIGNED, TOKENS> here, next;
+        uint4 k[2][KB];
+        uint4 v[4][VB];
+        float ks[4], vs[4];
+        auto token = [&](int i) { return i < 2 ? 2 * r + i : 6 + 2 * r + i; };     // the four tokens whose scores this lane holds
+        auto load_k = [&](const Places<ALIGNED, TOKENS>& at, int64_t base, int batch) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int page = at.page_of(g + 8 * i);
+                const unsigned slot = at.slot_of(g + 8 * i);
+                const int64_t t = base + g + 8 * i;
+                const bool in = page >= 0 && t >= range.first && t < range.n;
+                const char* row = kbase + page * p.kcs[0] + slot * p.kcs[2];
+#pragma unroll
+                for (int c = 0; c < KB; ++c) {
+                    const int byte = (batch * KB + c) * 64;
+                    k[i][c] = load16(row + byte, in && byte + r * 16 < p.d * ES);
+                }
+            }
+        };
+        auto load_v = [&](const Places<ALIGNED, TOKENS>& at, int64_t base, int batch) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int page = at.page_of(token(i));
+                const unsigned slot = at.slot_of(token(i));
+                const int64_t t = base + token(i);
+                const bool in = page >= 0 && t >= range.first && t < range.n;
+                const char* row = vbase + page * p.vcs[0] + slot * p.vcs[2];
+#pragma unroll
+                for (int c = 0; c < VB; ++c) {
+                    const int byte = (batch * VB + c) * 8 * VW;
+                    const bool wanted = in && byte + g * VW < p.d * ES;
+                    if constexpr (VW == 16) {
+                        v[i][c] = load16(row + byte, wanted);
+                    } else {
+                        uint2 w = make_uint2(0u, 0u);
+                        if (wanted) w = __ldg(reinterpret_cast<const uint2*>(row + byte));
+                        v[i][c] = make_uint4(w.x, w.y, 0u, 0u);
+                    }
+                }
+            }
+        };
+        auto load_scales = [&](const Places<ALIGNED, TOKENS>& at, int64_t base) {
+            if constexpr (E4M3) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int page = at.page_of(token(i));
+                    const unsigned slot = at.slot_of(token(i));
+                    const int64_t t = base + token(i);
+                    const bool in = page >= 0 && t >= range.first && t < range.n;
+                    const int64_t o = page * p.ss[0] + s.kv_head * p.ss[1] + slot * p.ss[2];
+                    ks[i] = in ? __ldg(p.k_scale + o) : 1.0f;
+                    vs[i] = in ? __ldg(p.v_scale + o) : 1.0f;
+                }
+            }
+        };
+        if (t0 < t_end) {
+            here.fetch(p, table, t0, lane, range.n);
+            next.fetch(p, table, t0 + STEP, lane, range.n);
+            here.settle(p, t0, lane, range);
+            load_k(here, t0, 0);
+            load_scales(here, t0);
+            load_v(here, t0, 0);
+        }
+        for (; t0 < t_end; t0 += STEP) {
+            const int64_t t1 = t0 + STEP;
+            const bool more = t1 < t_end;
+            // ---- scores
+            float sc[2][4] = {};
+#pragma unroll
+            for (int b = 0; b < KG / KB; ++b) {
+#pragma unroll
+                for (int c = 0; c < KB; ++c) {
+                    constexpr int QUARTER = KG * 32 * 4;
+                    const uint4* w = reinterpret_cast<const uint4*>(words + ((b * KB + c) * 32 + lane) * 4);
+                    if constexpr (E4M3) {
+                        const uint4 h0 = w[0], h1 = w[QUARTER / 4], l0 = w[2 * QUARTER / 4], l1 = w[3 * QUARTER / 4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint4 x = k[i][c];
+                            mma_f16(sc[i], h0.x, l0.x, h0.y, l0.y, half_of_e4m3(x.x), half_of_e4m3(x.x >> 16));
+                            mma_f16(sc[i], h0.z, l0.z, h0.w, l0.w, half_of_e4m3(x.y), half_of_e4m3(x.y >> 16));
+                            mma_f16(sc[i], h1.x, l1.x, h1.y, l1.y, half_of_e4m3(x.z), half_of_e4m3(x.z >> 16));
+                            mma_f16(sc[i], h1.z, l1.z, h1.w, l1.w, half_of_e4m3(x.w), half_of_e4m3(x.w >> 16));
+                        }
+                    } else {
+                        const uint4 hi = w[0], mid = w[QUARTER / 4], lo = w[2 * QUARTER / 4];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint4 x = k[i][c];
+                            mma_bf16(sc[i], hi.x, mid.x, hi.y, mid.y, x.x, x.y);
+                            mma_bf16(sc[i], lo.x, 0u, lo.y, 0u, x.x, x.y);
+                            mma_bf16(sc[i], hi.z, mid.z, hi.w, mid.w, x.z, x.w);
+                            mma_bf16(sc[i], lo.z, 0u, lo.w, 0u, x.z, x.w);
+                        }
+                    }
+                }
+                if (b + 1 < KG / KB) load_k(here, t0, b + 1);
+            }
+            // ---- the next tokens' keys
+            if (more) {
+                next.settle(p, t1, lane, range);
+                load_k(next, t1, 0);
+            }
+            // ---- weights
+            float w[4], top = -INFINITY, topv = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int64_t t = t0 + token(i);
+                const int page = here.page_of(token(i));          // (all lanes take part)
+                const bool seen = page >= 0 && t >= range.first && t < range.n;
+                float x = (sc[i / 2][i % 2] + sc[i / 2][2 + i % 2]) * unit;
+                if constexpr (E4M3) x *= ks[i];
+                w[i] = seen ? x : -INFINITY;
+                top = fmaxf(top, w[i]);
+            }
+            float sum = 0.0f;
+            if constexpr (E4M3) {
+                // the values' scales go into their weights: 2^e, e from the exponent field
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vs[i] = w[i] + (float)((int)(__float_as_uint(vs[i]) >> 23) - 127);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) topv = fmaxf(topv, vs[i]);
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            top = fmaxf(top, m);
+            const float base = settled(top);
+            float keep = exp2f(m - base);
+            l *= keep;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = exp2f(w[i] - base);
+                sum += e;
+                if constexpr (!E4M3) w[i] = e;
+            }
+            l += sum;
+            bool moved = top != m;
+            m = top;
+            if constexpr (E4M3) {
+                topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 1));
+                topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 2));
+                topv = fmaxf(topv, mv);
+                const float basev = settled(topv);
+                keep = exp2f(mv - basev);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = exp2f(vs[i] - basev + LIFT);
+                moved = topv != mv;
+                mv = topv;
+                if (more) load_scales(next, t1);
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int i = 0; i < VC * VE; ++i) {
+                    acc[i][0] *= keep; acc[i][1] *= keep; acc[i][2] *= keep; acc[i][3] *= keep;
+                }
+            }
+            unsigned a[6];
+            if constexpr (E4M3) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    a[i] = pack_half(w[2 * i], w[2 * i + 1]);
+                    const float2 f = unpack_half(a[i]);
+                    a[2 + i] = pack_half(w[2 * i] - f.x, w[2 * i + 1] - f.y);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float x = w[2 * i], y = w[2 * i + 1];
+                    a[i] = pack_bf16(x, y);
+                    x -= bf16_lo(a[i]);
+                    y -= bf16_hi(a[i]);
+                    a[2 + i] = pack_bf16(x, y);
+                    a[4 + i] = pack_bf16(x - bf16_lo(a[2 + i]), y - bf16_hi(a[2 + i]));
+                }
+            }
+            // ---- values
+#pragma unroll
+            for (int b = 0; b < VC / VB; ++b) {
+#pragma unroll
+                for (int c = 0; c < VB; ++c) {
+                    const int n0 = (b * VB + c) * VE;
+                    const unsigned x[4][4] = {{v[0][c].x, v[0][c].y, v[0][c].z, v[0][c].w}, {v[1][c].x, v[1][c].y, v[1][c].z, v[1][c].w},
+                                              {v[2][c].x, v[2][c].y, v[2][c].z, v[2][c].w}, {v[3][c].x, v[3][c].y, v[3][c].z, v[3][c].w}};
+#pragma unroll
+                    for (int i = 0; i < VW / 4; ++i) {
+                        if constexpr (E4M3) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const unsigned y0 = __byte_perm(x[0][i], x[1][i], e ? 0x7362 : 0x5140), y1 = __byte_perm(x[2][i], x[3][i], e ? 0x7362 : 0x5140);
+                                mma_f16(acc[n0 + 4 * i + 2 * e], a[0], a[2], a[1], a[3], half_of_e4m3(y0), half_of_e4m3(y1));
+                                mma_f16(acc[n0 + 4 * i + 2 * e + 1], a[0], a[2], a[1], a[3], half_of_e4m3(y0 >> 16), half_of_e4m3(y1 >> 16));
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const unsigned y0 = __byte_perm(x[0][i], x[1][i], e ? 0x7632 : 0x5410), y1 = __byte_perm(x[2][i], x[3][i], e ? 0x7632 : 0x5410);
+                                mma_bf16(acc[n0 + 2 * i + e], a[0], a[2], a[1], a[3], y0, y1);
+                                mma_bf16(acc[n0 + 2 * i + e], a[4], 0u, a[5], 0u, y0, y1);
+                            }
+                        }
+                    }
+                }
+                if (b + 1 < VC / VB) load_v(here, t0, b + 1);
+            }
+            if (more) {
+                load_v(next, t1, 0);
+                here = next;
+                next.fetch(p, table, t1 + STEP, lane, range.n);
+            }
+        }
+        // one sum per head, and e4m3 sums measured against m like the others
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        const float back = E4M3 ? exp2f(settled(mv) - settled(m) - LIFT) : 1.0f;
+#pragma unroll
+        for (int i = 0; i < VC * VE; ++i) {
+            acc[i][0] = (acc[i][0] + acc[i][2]) * back;
+            acc[i][1] = (acc[i][1] + acc[i][3]) * back;
+        }
+    }
+
+    // This warp's sums into shared memory: acc [HEADS][DP], ml [HEADS].
+    __device__ void put(float* out, float2* ml) const {
+        const int lane = threadIdx.x % 32, g = lane / 4, r = lane % 4;
+        if (r == 0) ml[g] = make_float2(m, l);
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int j = 0; j < VE; ++j) {
+                float* at = out + g * DP + c * 8 * VE + 2 * r * VE + j;
+                at[0] = acc[c * VE + j][0];
+                at[VE] = acc[c * VE + j][1];
+            }
+    }
+};
+
+// ------------------------------------------------------------------------------------------------------ FP32 cache
+// One warp's share of a segment with FP32 FMAs, HT heads at once.  Scores: lane (g, r) holds 16-byte pieces r, r + 4, .. of
+// token g's key (and of token 8 + g's), and four lanes add up to a score.  Values: the lanes lie along d, and the weights
+// come back through a few words of shared memory.
+template <int DP, int HT>
+struct FmaWarp {
+    static constexpr int HEADS = HT;
+    static constexpr int TOKENS = DP <= 64 ? 16 : 8;
+    static constexpr int TG = TOKENS / 8;                  // tokens whose keys a lane holds parts of
+    static constexpr int KC = DP / 16;                     // 16-byte pieces of a key a lane holds
+    static constexpr int LPT = DP / 4 < 32 ? DP / 4 : 32;  // lanes along a value
+    static constexpr int TPI = 32 / LPT;                   // tokens per load instruction
+    static constexpr int VC = DP / 4 / LPT;                // pieces of a value a lane holds
+    static constexpr int VI = TOKENS / TPI;
+    static constexpr int OWN = (HT + 3) / 4;               // heads whose weights a lane computes
+    static constexpr int Q_BYTES = HT * DP * 4;
+    static constexpr int W_BYTES = (TOKENS * HT + HT) * 8; // per warp: weights and factors, doubled for two FMAs at once
+
+    static __device__ void stage_queries(const AttnParams& p, const Segment& s, float* words) {
+        const float* q = p.q + s.row * p.qs[0] + s.head0 * p.qs[1];
+        for (int i = threadIdx.x; i < HT * DP; i += THREADS) {
+            const int h = i / DP, c = i % DP;
+            words[i] = h < s.heads && c < p.d ? q[h * p.qs[1] + c] : 0.0f;
+        }
+    }
+
+    unsigned long long acc[HT][VC][2];
+    float m[OWN], l[OWN];          // of heads r, r + 4 (modulo HT); l over this lane's tokens only
+
+    template <bool ALIGNED>
+    __device__ void run(const AttnParams& p, const Segment& s, const float* q, unsigned long long* weights, int64_t tile, int64_t tile_end) {
+        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, r = lane % 4;
+        const int64_t* table = p.page_table + s.row * p.table_stride;
+        const RowRange range = s.range;
+        constexpr int64_t STEP = WARPS * TOKENS;
+        int64_t t0 = tile * STEP + warp * TOKENS;
+        const int64_t t_end = tile_end * STEP;
+        unsigned long long* factors = weights + TOKENS * HT;
+#pragma unroll
+        for (int h = 0; h < HT; ++h)
+#pragma unroll
+            for (int c = 0; c < VC; ++c) acc[h][c][0] = acc[h][c][1] = 0ull;
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
+        const char* kbase = p.kc + s.kv_head * p.kcs[1] + r * 16;
+        const int along = lane % LPT, which = lane / LPT;
+        const char* vbase = p.vc + s.kv_head * p.vcs[1] + along * 16;
+        const float unit = p.scale * LOG2E;
+        Places<ALIGNED, TOKENS> here, next;
+        uint4 k[TG][KC];
+        uint4 v[VI][VC];
+        auto load_k = [&](const Places<ALIGNED, TOKENS>& at, int64_t base) {
+#pragma unroll
+            for (int i = 0; i < TG; ++i) {
+                const int page = at.page_of(g + 8 * i);
+                const unsigned slot = at.slot_of(g + 8 * i);
+                const int64_t t = base + g + 8 * i;
+                const bool in = page >= 0 && t >= range.first && t < range.n;
+                const char* row = kbase + page * p.kcs[0] + slot * p.kcs[2];
+#pragma unroll
+                for (int c = 0; c < KC; ++c) k[i][c] = load16(row + c * 64, in && c * 64 + r * 16 < p.d * 4);
+            }
+        };
+        auto load_v = [&](const Places<ALIGNED, TOKENS>& at, int64_t base) {
+#pragma unroll
+            for (int i = 0; i < VI; ++i) {
+                const int tk = i * TPI + which;
+                const int page = at.page_of(tk);
+                const unsigned slot = at.slot_of(tk);
+                const int64_t t = base + tk;
+                const bool in = page >= 0 && t >= range.first && t < range.n;
+                const char* row = vbase + page * p.vcs[0] + slot * p.vcs[2];
+#pragma unroll
+                for (int c = 0; c < VC; ++c) v[i][c] = load16(row + c * 512, in && c * 512 + along * 16 < p.d * 4);
+            }
+        };
+        if (t0 < t_end) {
+            here.fetch(p, table, t0, lane, range.n);
+            next.fetch(p, table, t0 + STEP, lane, range.n);
+            here.settle(p, t0, lane, range);
+            load_k(here, t0);
+            load_v(here, t0);
+        }
+        for (; t0 < t_end; t0 += STEP) {
+            const int64_t t1 = t0 + STEP;
+            const bool more = t1 < t_end;
+            // ---- scores: every lane of a quad ends with the sums of all heads
+            float sc[TG][HT];
+#pragma unroll
+            for (int h = 0; h < HT; ++h) {
+                unsigned long long part[TG][2];
+#pragma unroll
+                for (int i = 0; i < TG; ++i) part[i][0] = part[i][1] = 0ull;
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    const ulonglong2 qq = *reinterpret_cast<const ulonglong2*>(q + h * DP + c * 16 + r * 4);
+#pragma unroll
+                    for (int i = 0; i < TG; ++i) {
+                        const ulonglong2 kk = *reinterpret_cast<const ulonglong2*>(&k[i][c]);
+                        fma2(part[i][0], qq.x, kk.x);
+                        fma2(part[i][1], qq.y, kk.y);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < TG; ++i) {
+                    const float2 x = unpair(part[i][0]), y = unpair(part[i][1]);
+                    sc[i][h] = (x.x + x.y) + (y.x + y.y);
+                }
+            }
+            if (more) {
+                next.settle(p, t1, lane, range);
+                load_k(next, t1);
+            }
+#pragma unroll
+            for (int i = 0; i < TG; ++i)
+#pragma unroll
+                for (int h = 0; h < HT; ++h) {
+                    sc[i][h] += __shfl_xor_sync(0xffffffffu, sc[i][h], 1);
+                    sc[i][h] += __shfl_xor_sync(0xffffffffu, sc[i][h], 2);
+                }
+            // ---- weights of heads r, r + 4 over tokens g (and 8 + g)
+            bool moved = false;
+#pragma unroll
+            for (int j = 0; j < OWN; ++j) {
+                const int h = (r + 4 * j) % HT;
+                float w[TG], top = m[j];
+#pragma unroll
+                for (int i = 0; i < TG; ++i) {
+                    float x = sc[i][(4 * j) % HT];
+#pragma unroll
+                    for (int u = 1; u < 4; ++u) x = r == u ? sc[i][(u + 4 * j) % HT] : x;
+                    const int64_t t = t0 + g + 8 * i;
+                    const int page = here.page_of(g + 8 * i);      // (all lanes take part)
+                    const bool seen = page >= 0 && t >= range.first && t < range.n;
+                    w[i] = seen ? x * unit : -INFINITY;
+                    top = fmaxf(top, w[i]);
+                }
+#pragma unroll
+                for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const float base = settled(top), keep = exp2f(m[j] - base);
+                l[j] *= keep;
+                moved |= top != m[j];
+                m[j] = top;
+#pragma unroll
+                for (int i = 0; i < TG; ++i) {
+                    const float e = exp2f(w[i] - base);
+                    l[j] += e;
+                    weights[(g + 8 * i) * HT + h] = pair(e, e);
+                }
+                if (g == 0) factors[h] = pair(keep, keep);
+            }
+            moved = __any_sync(0xffffffffu, moved);
+            __syncwarp();
+            if (moved) {
+#pragma unroll
+                for (int h = 0; h < HT; ++h) {
+                    const unsigned long long f = factors[h];
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+                        acc[h][c][0] = mul2(acc[h][c][0], f);
+                        acc[h][c][1] = mul2(acc[h][c][1], f);
+                    }
+                }
+            }
+            // ---- values
+#pragma unroll
+            for (int i = 0; i < VI; ++i) {
+                const unsigned long long* w = weights + (i * TPI + which) * HT;
+#pragma unroll
+                for (int h = 0; h < HT; ++h) {
+                    const unsigned long long x = w[h];
+#pragma unroll
+                    for (int c = 0; c < VC; ++c) {
+                        const ulonglong2 vv = *reinterpret_cast<const ulonglong2*>(&v[i][c]);
+                        fma2(acc[h][c][0], x, vv.x);
+                        fma2(acc[h][c][1], x, vv.y);
+                    }
+                }
+            }
+            __syncwarp();
+            if (more) {
+                load_v(next, t1);
+                here = next;
+                next.fetch(p, table, t1 + STEP, lane, range.n);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < OWN; ++j)
+#pragma unroll
+            for (int o = 4; o < 32; o *= 2) l[j] += __shfl_xor_sync(0xffffffffu, l[j], o);
+        // lanes that hold other tokens of the same elements
+#pragma unroll
+        for (int o = LPT; o < 32; o *= 2)
+#pragma unroll
+            for (int h = 0; h < HT; ++h)
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 x = unpair(acc[h][c][i]);
+                        acc[h][c][i] = pair(x.x + __shfl_xor_sync(0xffffffffu, x.x, o), x.y + __shfl_xor_sync(0xffffffffu, x.y, o));
+                    }
+    }
+
+    __device__ void put(float* out, float2* ml) const {
+        const int lane = threadIdx.x % 32, g = lane / 4, r = lane % 4;
+#pragma unroll
+        for (int j = 0; j < OWN; ++j)
+            if (g == 0 && r + 4 * j < HT) ml[r + 4 * j] = make_float2(m[j], l[j]);
+        if (lane < LPT) {
+#pragma unroll
+            for (int h = 0; h < HT; ++h)
+#pragma unroll
+                for (int c = 0; c < VC; ++c) {
+                    ulonglong2 x;
+                    x.x = acc[h][c][0];
+                    x.y = acc[h][c][1];
+                    *reinterpret_cast<ulonglong2*>(out + h * DP + c * 128 + lane * 4) = x;
+                }
+        }
+    }
+};
+
+template <int DTYPE, int DP, int HT> struct WarpOf { typedef TensorWarp<DTYPE, DP> type; };
+template <int DP, int HT> struct WarpOf<TE_KV_F32, DP, HT> { typedef FmaWarp<DP, HT> type; };
+
+// ---------------------------------------------------------------------------------------------------- the two kernels
+template <int DTYPE, int DP, int HT, bool ALIGNED>
+__global__ void __launch_bounds__(THREADS, 2) paged_attention_kernel(const AttnParams p) {
+    typedef typename WarpOf<DTYPE, DP, HT>::type Warp;
+    constexpr int HEADS = Warp::HEADS, TILE = WARPS * Warp::TOKENS;
+    __shared__ __align__(16) char query[Warp::Q_BYTES];
+    // the warps' sums at a segment's end; FP32 weights while it runs
+    __shared__ __align__(16) float sums[WARPS][HEADS][DP];
+    __shared__ float2 ml[WARPS][HEADS];
+    __shared__ float q_unit[HEADS];
+    __shared__ int64_t scan[WARPS];
+    __shared__ int64_t found_prefix;
+    __shared__ int found_row;
+    griddep_wait();
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    const int w = blockIdx.x;
+    const int tiles_of_heads = p.kv_heads * p.head_tiles;
+    const int64_t most = p.max_pages * (int64_t)p.page_size.divisor;
+
+    // ---- this worker's share: the rows' tile counts, added up by all threads over slabs of rows
+    const int slab = (p.rows + THREADS - 1) / THREADS;
+    const int r0 = min(p.rows, tid * slab), r1 = min(p.rows, r0 + slab);
+    int64_t mine = 0;
+    bool cut = false;
+    for (int r = r0; r < r1; ++r) {
+        const int64_t len = p.lens[r];
+        cut |= len > most;
+        mine += row_tiles(row_range(len, most, p.window), TILE);
+    }
+    if (cut) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
+    int64_t before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+    }
+    if (lane == 31) scan[warp] = before;
+    if (tid == 0) found_row = -1;
+    __syncthreads();
+    int64_t total = 0;
+    before -= mine;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+        if (i < warp) before += scan[i];
+        total += scan[i];
+    }
+    const int64_t units = total * tiles_of_heads;
+    const int workers = (int)(units < gridDim.x ? units : (int64_t)gridDim.x);      // every one of them has a unit
+    int64_t unit = w < workers ? worker_begin(units, workers, w) : 0;
+    const int64_t unit_end = w < workers ? worker_begin(units, workers, w + 1) : 0;
+    if (unit < unit_end) {
+        const int64_t at = unit / tiles_of_heads;          // in tiles of rows
+        if (at >= before && at < before + mine) {
+            for (int r = r0; r < r1; ++r) {
+                const int c = row_tiles(row_range(p.lens[r], most, p.window), TILE);
+                if (at < before + c) {
+                    found_row = r;
+                    found_prefix = before;
+                    break;
+                }
+                before += c;
+            }
+        }
+    }
+    if (tid == 0) p.joins[w] = make_int4(0, 0, 0, 0);
+    __syncthreads();
+    // rows without tokens
+    for (int r = w; r < p.rows; r += gridDim.x) {
+        if (row_tiles(row_range(p.lens[r], most, p.window), TILE) > 0) continue;
+        for (int i = tid; i < p.q_heads * p.d; i += THREADS) p.o[r * p.os[0] + i / p.d * p.os[1] + i % p.d] = 0.0f;
+        if (p.lse)
+            for (int i = tid; i < p.q_heads; i += THREADS) p.lse[(int64_t)r * p.q_heads + i] = -INFINITY;
+    }
+    if (unit >= unit_end) return;
+
+    // ---- its segments
+    int row = found_row;
+    int64_t row_begin = found_prefix * tiles_of_heads;     // first unit of the row
+    while (unit < unit_end) {
+        Segment s;
+        s.row = row;
+        s.range = row_range(p.lens[row], most, p.window);
+        const int tiles = row_tiles(s.range, TILE);
+        if (tiles == 0) { ++row; continue; }
+        const int64_t in_row = unit - row_begin;
+        const int ht = (int)(in_row / tiles);
+        if (ht >= tiles_of_heads) {
+            row_begin += (int64_t)tiles * tiles_of_heads;
+            ++row;
             continue;
         }
-        const int64_t ka = page * p.kcs[0] + kh * p.kcs[1] + slot * p.kcs[2], va = page * p.vcs[0] + kh * p.vcs[1] + slot * p.vcs[2];
-        float sk = 1.0f, sv = 1.0f;
-        if constexpr (DTYPE == TE_KV_E4M3) {
-            const int64_t s = page * p.ss[0] + kh * p.ss[1] + slot * p.ss[2];
-            sk = p.k_scale[s];
-            sv = p.v_scale[s];
+        const int64_t seg_begin = row_begin + (int64_t)ht * tiles, seg_end = seg_begin + tiles;
+        const int64_t stop = unit_end < seg_end ? unit_end : seg_end;
+        s.kv_head = ht / p.head_tiles;
+        const int part = ht % p.head_tiles * HEADS;
+        s.head0 = s.kv_head * p.group + part;
+        s.heads = min(HEADS, p.group - part);
+        const int64_t tile0 = s.range.first / TILE + (unit - seg_begin), tile1 = s.range.first / TILE + (stop - seg_begin);
+        {
+            Warp mywarp;
+            if constexpr (DTYPE == TE_KV_F32) {
+                Warp::stage_queries(p, s, reinterpret_cast<float*>(query));
+                __syncthreads();
+                // the weights' words lie where this warp's own sums will go
+                static_assert(Warp::W_BYTES <= sizeof(sums[0]), "weights fit the warp's sums");
+                mywarp.template run<ALIGNED>(p, s, reinterpret_cast<const float*>(query), reinterpret_cast<unsigned long long*>(sums[warp]), tile0, tile1);
+                __syncwarp();
+            } else {
+                Warp::stage_queries(p, s, reinterpret_cast<unsigned*>(query), q_unit);
+                __syncthreads();
+                mywarp.template run<ALIGNED>(p, s, reinterpret_cast<const unsigned*>(query), q_unit, tile0, tile1);
+            }
+            mywarp.put(&sums[warp][0][0], ml[warp]);
         }
-        float s = 0.0f;
+        __syncthreads();
+        // ---- the four warps' sums into the result, or into the workspace when the segment is shared with other workers
+        const bool whole = unit == seg_begin && stop == seg_end;
+        const int slot = part_slot(w, unit == seg_begin);
+        for (int i = tid; i < s.heads * (p.d / 4); i += THREADS) {
+            const int h = i / (p.d / 4), c = i % (p.d / 4) * 4;
+            float m = ml[0][h].x;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = lane + 32 * i;
-            if (i < per && c < p.d) s += q[i] * stored_value<DTYPE>(p.kc, ka + c);
+            for (int j = 1; j < WARPS; ++j) m = fmaxf(m, ml[j][h].x);
+            const float base = settled(m);
+            float l = 0.0f;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < WARPS; ++j) {
+                const float f = exp2f(ml[j][h].x - base);
+                const float4 x = *reinterpret_cast<const float4*>(&sums[j][h][c]);
+                l += f * ml[j][h].y;
+                a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
+            }
+            if (whole) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                float* o = p.o + s.row * p.os[0] + (s.head0 + h) * p.os[1] + c;
+                o[0] = a.x * inv; o[1] = a.y * inv; o[2] = a.z * inv; o[3] = a.w * inv;
+                if (p.lse && c == 0) p.lse[(int64_t)s.row * p.q_heads + s.head0 + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+            } else {
+                *reinterpret_cast<float4*>(p.part_acc + ((int64_t)slot * HEADS + h) * p.d + c) = a;
+                if (c == 0) p.part_ml[slot * HEADS + h] = make_float2(m, l);
+            }
         }
+        if (tid == 0 && unit == seg_begin && stop < seg_end) p.joins[w] = make_int4(s.row, ht, worker_of(units, workers, seg_end - 1), 1);
+        __syncthreads();
+        unit = stop;
+    }
+}
+
+// Adds the parts of the segment that begins in worker blockIdx.x's share, in the order of its tokens, for head blockIdx.y of
+// the tile: warps take parts in turn, lanes lie along d; then the warps' sums are added in order.
+constexpr int JOIN_WARPS = 8;
+__global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(const AttnParams p, int heads_per_tile) {
+    __shared__ float sums[JOIN_WARPS][256];
+    __shared__ float tops[JOIN_WARPS], totals[JOIN_WARPS];
+    griddep_wait();
+    const int w = blockIdx.x, h = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int4 j = p.joins[w];
+    if (!j.w) return;
+    const int kv_head = j.y / p.head_tiles, part = j.y % p.head_tiles * heads_per_tile;
+    if (part + h >= p.group) return;
+    const int count = j.z - w + 1;
+    auto at = [&](int i) { return (int64_t)part_slot(w + i, i == 0) * heads_per_tile + h; };
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < count; i += 32 * JOIN_WARPS) m = fmaxf(m, p.part_ml[at(i)].x);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        s *= sk;
-        const float top = fmaxf(m, s);
-        const float keep = m == top ? 1.0f : expf(m - top), w = s == top ? 1.0f : expf(s - top);
-        m = top;
-        l = l * keep + w;
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) tops[warp] = m;
+    __syncthreads();
+    m = tops[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = lane + 32 * i;
-            if (i < per && c < p.d) acc[i] = acc[i] * keep + w * (sv * stored_value<DTYPE>(p.vc, va + c));
+    for (int i = 1; i < JOIN_WARPS; ++i) m = fmaxf(m, tops[i]);
+    const float base = settled(m);
+    float a[8] = {}, l = 0.0f;
+#pragma unroll 4
+    for (int i = warp; i < count; i += JOIN_WARPS) {
+        const int64_t o = at(i);
+        const float2 ml = p.part_ml[o];
+        const float f = exp2f(ml.x - base);
+        l += f * ml.y;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int c = u * 128 + lane * 4;
+            if (c < p.d) {
+                const float4 x = *reinterpret_cast<const float4*>(p.part_acc + o * p.d + c);
+                a[4 * u] += f * x.x; a[4 * u + 1] += f * x.y; a[4 * u + 2] += f * x.z; a[4 * u + 3] += f * x.w;
+            }
         }
     }
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = lane + 32 * i;
-        if (i < per && c < p.d) p.o[r * p.os[0] + h * p.os[1] + c] = acc[i] * inv;
+    for (int u = 0; u < 8; ++u) sums[warp][u / 4 * 128 + lane * 4 + u % 4] = a[u];
+    if (lane == 0) totals[warp] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < JOIN_WARPS; ++i) l += totals[i];
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int head = kv_head * p.group + part + h;
+    for (int c = threadIdx.x; c < p.d; c += 32 * JOIN_WARPS) {
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < JOIN_WARPS; ++i) x += sums[i][c];
+        p.o[j.x * p.os[0] + head * p.os[1] + c] = x * inv;
     }
-    if (p.lse && lane == 0) p.lse[r * p.q_heads + h] = l == 0.0f ? -INFINITY : m + logf(l);
+    if (p.lse && threadIdx.x == 0) p.lse[(int64_t)j.x * p.q_heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
+// ------------------------------------------------------------------------------------------------------------ host side
+// Heads a tile holds: 8 on the tensor cores; with FMAs the smallest of 1, 2, 4, 8 that takes the group, since every head
+// of a tile is computed whether it is there or not.
+int heads_per_tile(int dtype, int64_t group) { return dtype != TE_KV_F32 ? 8 : group >= 5 ? 8 : group >= 3 ? 4 : (int)group; }
+
+// Thread blocks per SM: what the registers allow (two of 128 threads at up to 255 each).
+constexpr int BLOCKS_PER_SM = 2;
+
+size_t workspace_need(const te_paged_attn_desc* t, int sm_count) {
+    if (t->rows == 0 || t->q_heads == 0) return 0;
+    const size_t workers = (size_t)sm_count * BLOCKS_PER_SM, heads = heads_per_tile(t->cache.dtype, t->q_heads / t->cache.heads);
+    return workers * 16 + 2 * workers * heads * (8 + 4 * (size_t)t->cache.d);
+}
+
+template <int DTYPE, int DP, int HT>
+cudaError_t launch_tiles(const AttnParams& p, int workers, cudaStream_t st) {
+    const bool aligned = p.page_size.divisor % 16 == 0;       // a warp's 16 (or 8) tokens never straddle pages
+    return aligned ? launch_pdl(paged_attention_kernel<DTYPE, DP, HT, true>, dim3(workers), dim3(THREADS), 0, st, p)
+                   : launch_pdl(paged_attention_kernel<DTYPE, DP, HT, false>, dim3(workers), dim3(THREADS), 0, st, p);
+}
+
+template <int DP>
+cudaError_t launch_width(const AttnParams& p, int dtype, int heads, int workers, cudaStream_t st) {
+    if (dtype == TE_KV_BF16) return launch_tiles<TE_KV_BF16, DP, 8>(p, workers, st);
+    if (dtype == TE_KV_E4M3) return launch_tiles<TE_KV_E4M3, DP, 8>(p, workers, st);
+    if (heads == 1) return launch_tiles<TE_KV_F32, DP, 1>(p, workers, st);
+    if (heads == 2) return launch_tiles<TE_KV_F32, DP, 2>(p, workers, st);
+    if (heads == 4) return launch_tiles<TE_KV_F32, DP, 4>(p, workers, st);
+    return launch_tiles<TE_KV_F32, DP, 8>(p, workers, st);
 }
 
 int check_desc(const te_paged_attn_desc* t) {
@@ -116,6 +941,7 @@ int check_desc(const te_paged_attn_desc* t) {
     const te_kv_cache& c = t->cache;
     if (t->q_heads > 0 && (c.heads == 0 || t->q_heads % c.heads)) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: q_heads must be a multiple of the cache's heads");
     if (t->max_pages > 0 && c.page_size > INT32_MAX / t->max_pages) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: the page table reaches beyond 2^31-1 positions");
+    if (c.pages > INT32_MAX) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: more than 2^31-1 pages");
     if (t->q_heads > 65535 || (t->q_heads > 0 && t->rows > INT32_MAX / t->q_heads)) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: too many rows or heads");
     if (t->window < 0) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: negative window");
     if (!isfinite(t->scale)) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: scale must be finite");
@@ -139,7 +965,7 @@ extern "C" {
 int te_b200_paged_attention_workspace_size(const te_paged_attn_desc* d, int sm_count, size_t* out_bytes) {
     if (!out_bytes || sm_count < 1) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: out_bytes is NULL or sm_count not positive");
     if (int bad = check_desc(d)) return bad;
-    *out_bytes = 0;
+    *out_bytes = workspace_need(d, sm_count);
     return TE_OK;
 }
 
@@ -148,25 +974,39 @@ int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* t, te_st
     if (int bad = check_ctx(ctx)) return bad;
     if (t->rows == 0 || t->q_heads == 0) return TE_OK;
     const te_kv_cache& c = t->cache;
+    const size_t need = workspace_need(t, ctx->sm_count);
+    if (need > ctx->workspace_bytes) {
+        char msg[160];
+        snprintf(msg, sizeof msg, "context workspace (%zu bytes) too small; paged attention needs %zu bytes", ctx->workspace_bytes, need);
+        return fail(TE_ERR_WORKSPACE, msg);
+    }
+    const int workers = ctx->sm_count * BLOCKS_PER_SM;
     AttnParams p;
-    p.q = t->q; p.o = t->o; p.lse = t->lse; p.kc = c.k; p.vc = c.v; p.k_scale = c.k_scale; p.v_scale = c.v_scale;
+    p.q = t->q; p.o = t->o; p.lse = t->lse;
+    p.kc = static_cast<const char*>(c.k); p.vc = static_cast<const char*>(c.v); p.k_scale = c.k_scale; p.v_scale = c.v_scale;
     p.page_table = t->page_table; p.lens = t->lens;
+    const int64_t size = c.dtype == TE_KV_F32 ? 4 : c.dtype == TE_KV_BF16 ? 2 : 1;
     for (int i = 0; i < 2; ++i) { p.qs[i] = t->q_strides[i]; p.os[i] = t->o_strides[i]; }
-    for (int i = 0; i < 3; ++i) { p.kcs[i] = c.k_strides[i]; p.vcs[i] = c.v_strides[i]; p.ss[i] = c.scale_strides[i]; }
+    for (int i = 0; i < 3; ++i) { p.kcs[i] = c.k_strides[i] * size; p.vcs[i] = c.v_strides[i] * size; p.ss[i] = c.scale_strides[i]; }
     p.table_stride = t->page_table_stride; p.max_pages = t->max_pages; p.pages = c.pages; p.window = t->window;
-    p.rows = t->rows;
     p.page_size = make_fast_divisor((uint32_t)c.page_size);
-    p.q_heads = (int)t->q_heads; p.group = (int)(t->q_heads / c.heads); p.d = (int)c.d;
+    p.rows = (int)t->rows; p.q_heads = (int)t->q_heads; p.kv_heads = (int)c.heads;
+    p.group = (int)(t->q_heads / c.heads); p.d = (int)c.d;
+    const int heads = heads_per_tile(c.dtype, p.group);
+    p.head_tiles = (p.group + heads - 1) / heads;
     p.scale = t->scale;
+    char* ws = static_cast<char*>(ctx->workspace);
+    p.joins = reinterpret_cast<int4*>(ws);
+    p.part_ml = reinterpret_cast<float2*>(ws + (size_t)workers * 16);
+    p.part_acc = reinterpret_cast<float*>(ws + (size_t)workers * 16 + (size_t)workers * 2 * heads * 8);
     p.status = ctx->d_status;
-    const dim3 grid((unsigned)(t->rows * t->q_heads)), block(32);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e;
-    if (c.dtype == TE_KV_F32) e = launch_pdl(paged_attention_kernel<TE_KV_F32>, grid, block, 0, st, p);
-    else if (c.dtype == TE_KV_BF16) e = launch_pdl(paged_attention_kernel<TE_KV_BF16>, grid, block, 0, st, p);
-    else e = launch_pdl(paged_attention_kernel<TE_KV_E4M3>, grid, block, 0, st, p);
+    cudaError_t e = p.d <= 64 ? launch_width<64>(p, c.dtype, heads, workers, st) : p.d <= 128 ? launch_width<128>(p, c.dtype, heads, workers, st)
+                                                                                  : launch_width<256>(p, c.dtype, heads, workers, st);
     if (e != cudaSuccess) return cuda_fail(e, "paged_attention_kernel launch");
-    ctx->launches += 1;
+    e = launch_pdl(paged_join_kernel, dim3((unsigned)workers, (unsigned)heads), dim3(32 * JOIN_WARPS), 0, st, p, heads);
+    if (e != cudaSuccess) return cuda_fail(e, "paged_join_kernel launch");
+    ctx->launches += 2;
     return TE_OK;
 }
 
