@@ -8,15 +8,15 @@
 // * A fixed number of thread blocks, all resident, share the tiles of all rows evenly (paged_plan.h), so that one long
 //   sequence, many short ones and any mixture keep every SM reading.  A block that holds only part of a (row, head tile)
 //   leaves its sums in the workspace; paged_join_kernel adds the parts in their order.
-// * Keys and values go from global memory straight into the registers that the arithmetic reads, 16 bytes a lane, the next
-//   tokens' loads in flight during the arithmetic of the current ones; nothing is staged in shared memory.
+// * Every warp copies its own tokens into a ring of its own in shared memory, 16 bytes a lane with cp.async, two stages
+//   ahead of the one it computes on, and waits for nobody else until the segment ends.
 //
 // 2- and 1-byte caches use the tensor cores through mma.sync m16n8k16 (8 query rows do not fill the 128-row tiles of
 // tcgen05, and the products need 5 % of the tensor rate): a stored value is exactly a bf16 resp. half, and an FP32 query
 // or weight is exactly (to 2^-24 of its row's largest) the sum of three bf16 resp. two half terms, so that products and
 // sums are those of FP32.  The terms of a head occupy rows g and g + 8 of one tile, both in the same thread.  Which element of a head
-// an index of the contraction stands for is free as long as both operands agree, and chosen so that a lane's 16 bytes are
-// its operand.  An FP32 cache uses FP32 FMAs (two per instruction).
+// an index of the contraction stands for is free as long as both operands agree, and chosen so that a lane's operand is 16
+// bytes of a row as it lies in the cache.  An FP32 cache uses FP32 FMAs (two per instruction).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -90,11 +90,20 @@ __device__ __forceinline__ unsigned half_of_e4m3(unsigned two) {
     asm("{ .reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t; }" : "=r"(r) : "r"(two));
     return r;
 }
-__device__ __forceinline__ uint4 load16(const char* p, bool there) {
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (there) v = __ldg(reinterpret_cast<const uint4*>(p));
-    return v;
+__device__ __forceinline__ unsigned smem_address(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(unsigned to, const char* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+// Zeros where !there (nothing is read then).
+__device__ __forceinline__ void copy16_or_zero(unsigned to, const char* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4_or_zero(unsigned to, const float* from, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ unsigned long long pair(float x, float y) {
     unsigned long long v;
     asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
@@ -116,52 +125,167 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
 // exp2 of a score less the maximum; a maximum of -infinity means that nothing has been seen.
 __device__ __forceinline__ float settled(float m) { return m == -INFINITY ? 0.0f : m; }
 
-// The pages that hold N consecutive tokens from t0 (a multiple of N).  ALIGNED: one page holds them all.
-template <bool ALIGNED, int N>
-struct Places {
-    int64_t entry;     // as read, of token (lane & (N - 1)) resp. of all
-    int page;
-    unsigned slot;
-    __device__ __forceinline__ void fetch(const AttnParams& p, const int64_t* table, int64_t t0, int lane, int64_t n) {
-        const int64_t t = ALIGNED ? t0 : t0 + (lane & (N - 1));
-        entry = -1;
-        slot = 0;
-        if (t < n) {                       // n is within the table
-            const unsigned i = fast_quotient((unsigned)t, p.page_size);
-            slot = (unsigned)t - i * p.page_size.divisor;
-            entry = __ldg(table + i);
+// A warp's ring: stages of TOKENS rows of keys and as many of values (and their scales), DP elements of ES bytes a row.
+//
+// PACKED: pages are multiples of 16 slots, rows of a page and head lie one behind the other, and d == DP.  Sixteen tokens
+// are then one contiguous piece, and a stage's copies are immediate offsets from a few page addresses.  Otherwise every
+// token's place is looked up by the lane of its number and handed round, and what a row lacks to DP elements is zero-filled.
+//
+// Rows are multiples of 128 bytes apart (of 64 for DP = 64 bytes), so lanes that read different rows would meet in the
+// same banks.  16-byte pieces are therefore exchanged within a row by an exclusive-or with bits of the row's number:
+// readers of keys take pieces 4c .. 4c + 3 of rows 2i and 2i + 1 at a time, readers of values pieces 2c, 2c + 1 of every
+// other row of eight.
+template <int DP, int ES, int TOKENS_, int STAGES_, bool SCALES, bool PACKED>
+struct Ring {
+    static constexpr int TOKENS = TOKENS_, STAGES = STAGES_;
+    static constexpr int RB = DP * ES;                                 // bytes of a row
+    static constexpr int CPR = RB / 16;                                // pieces of a row
+    static constexpr int TPI = CPR >= 32 ? 1 : 32 / CPR;               // rows a warp copies at once
+    static constexpr int PPR = CPR >= 32 ? CPR / 32 : 1;               // copies a lane makes of a row
+    static constexpr int SIDE = TOKENS * RB;                           // bytes of the keys, and of the values, of a stage
+    static constexpr int STAGE = 2 * SIDE + (SCALES ? 2 * TOKENS * 4 : 0);
+    static constexpr int BYTES = STAGE * STAGES;
+    static constexpr int STEP = WARPS * TOKENS;                        // from one of a warp's stages to its next
+    static constexpr int BLOCK = TOKENS < 16 ? TOKENS : 16;            // tokens of one page lookup
+    static constexpr int NB = PACKED ? TOKENS / BLOCK : 1;
+
+    // Byte offset of piece j of row t.
+    static __device__ __forceinline__ int key_at(int t, int j) {
+        return RB == 64 ? ((t * 4 + j) ^ ((t >> 1 & 1) << 1) ^ ((t >> 2 & 1) << 2)) * 16 : t * RB + (j ^ ((t & 1) << 2)) * 16;
+    }
+    static __device__ __forceinline__ int value_at(int t, int j) {
+        if constexpr (ES == 4) return t * RB + j * 16;                 // lanes read along a row
+        return RB == 64 ? key_at(t, j) : t * RB + (j ^ ((t >> 1 & 3) << 1)) * 16;
+    }
+
+    unsigned base;              // shared-memory address of the ring
+    int64_t entry[NB];          // of the page table, as read, for the stage to be issued next
+    unsigned slot[NB];
+
+    __device__ __forceinline__ const char* stage(const char* ring, int i) const { return ring + i * STAGE; }
+
+    // Reads the page table for the tokens from t0 on; lane's own token (!PACKED), or the page of each block.
+    __device__ __forceinline__ void look_up(const AttnParams& p, const int64_t* table, int64_t t0, int64_t t_end, int64_t n) {
+        const int lane = threadIdx.x % 32;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int64_t t = t0 + (PACKED ? b * BLOCK : lane % TOKENS);
+            entry[b] = -1;
+            slot[b] = 0;
+            if (t0 < t_end && t < n) {                 // n is within the table
+                const unsigned i = fast_quotient((unsigned)t, p.page_size);
+                slot[b] = (unsigned)t - i * p.page_size.divisor;
+                entry[b] = __ldg(table + i);
+            }
         }
     }
-    // Checks what fetch read; reports a page outside the cache that a token of [first, n) lies in.
-    __device__ __forceinline__ void settle(const AttnParams& p, int64_t t0, int lane, const RowRange& range) {
-        const bool good = entry >= 0 && entry < p.pages;
-        page = good ? (int)entry : -1;
-        const int64_t t = ALIGNED ? t0 : t0 + (lane & (N - 1));
-        if (!good && t < range.n && (ALIGNED ? t + N > range.first : t >= range.first)) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
+
+    // Issues the copies of the tokens from t0 on, whose places look_up has read, into stage i.  Returns which of them may be
+    // attended to: bit t for token t0 + t.
+    __device__ __forceinline__ unsigned issue(const AttnParams& p, const RowRange& range, int kv_head, int64_t t0, int i) {
+        const int lane = threadIdx.x % 32;
+        const unsigned to = base + i * STAGE;
+        const int chunk = lane % (CPR < 32 ? CPR : 32), sub = CPR >= 32 ? 0 : lane / CPR;
+        const char* kc = p.kc + kv_head * p.kcs[1];
+        const char* vc = p.vc + kv_head * p.vcs[1];
+        // tokens inside the range, then those on pages of the cache
+        const int64_t lo = range.first - t0, hi = range.n - t0;
+        unsigned seen = hi <= 0 ? 0u : hi >= TOKENS ? 0xffffffffu >> (32 - TOKENS) : (1u << hi) - 1u;
+        if (lo > 0) seen = lo >= TOKENS ? 0u : seen & ~((1u << lo) - 1u);
+        unsigned good = 0u;
+        if constexpr (PACKED) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                if (entry[b] >= 0 && entry[b] < p.pages) good |= (BLOCK == 16 ? 0xffffu : 0xffu) << (b * BLOCK);
+        } else {
+            good = __ballot_sync(0xffffffffu, entry[0] >= 0 && entry[0] < p.pages);
+        }
+        if (seen & ~good) {
+            if (lane == 0) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
+            seen &= good;
+        }
+        if constexpr (PACKED) {
+            const bool all = seen == 0xffffffffu >> (32 - TOKENS);
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const bool there = (good >> (b * BLOCK)) & 1u;
+                const char* k = kc + (there ? entry[b] * p.kcs[0] + slot[b] * (int64_t)RB : 0) + lane * 16;
+                const char* v = vc + (there ? entry[b] * p.vcs[0] + slot[b] * (int64_t)RB : 0) + lane * 16;
+#pragma unroll
+                for (int c = 0; c < BLOCK / TPI; ++c)
+#pragma unroll
+                    for (int u = 0; u < PPR; ++u) {
+                        const int t = b * BLOCK + c * TPI + sub;
+                        const unsigned kd = to + key_at(t, chunk + 32 * u), vd = to + SIDE + value_at(t, chunk + 32 * u);
+                        const int o = (c * PPR + u) * 512;
+                        if (all) {
+                            copy16(kd, k + o);
+                            copy16(vd, v + o);
+                        } else {
+                            copy16_or_zero(kd, k + o, seen >> t & 1u);
+                            copy16_or_zero(vd, v + o, seen >> t & 1u);
+                        }
+                    }
+            }
+        } else {
+            const int page = good >> lane & 1u ? (int)entry[0] : 0;
+#pragma unroll
+            for (int c = 0; c < TOKENS / TPI; ++c) {
+                const int t = c * TPI + sub;
+                const int64_t at = __shfl_sync(0xffffffffu, page, t);
+                const int64_t in = __shfl_sync(0xffffffffu, slot[0], t);
+                const char* k = kc + at * p.kcs[0] + in * p.kcs[2];
+                const char* v = vc + at * p.vcs[0] + in * p.vcs[2];
+#pragma unroll
+                for (int u = 0; u < PPR; ++u) {
+                    const int j = chunk + 32 * u;
+                    const bool there = (seen >> t & 1u) && j * 16 < p.d * ES;
+                    copy16_or_zero(to + key_at(t, j), k + (there ? j * 16 : 0), there);
+                    copy16_or_zero(to + SIDE + value_at(t, j), v + (there ? j * 16 : 0), there);
+                }
+            }
+        }
+        if constexpr (SCALES) {          // lane t copies token t's
+            int64_t at = 0;
+            const bool mine = lane < TOKENS && (seen >> (lane % TOKENS) & 1u);
+            if constexpr (PACKED) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+                    if (lane / BLOCK == b) at = entry[b] * p.ss[0] + (int64_t)(slot[b] + lane % BLOCK) * p.ss[2];
+            } else {
+                at = entry[0] * p.ss[0] + (int64_t)slot[0] * p.ss[2];
+            }
+            at = mine ? at + kv_head * p.ss[1] : 0;
+            if (lane < TOKENS) {
+                copy4_or_zero(to + 2 * SIDE + lane * 4, p.k_scale + at, mine);
+                copy4_or_zero(to + 2 * SIDE + TOKENS * 4 + lane * 4, p.v_scale + at, mine);
+            }
+        }
+        return seen;
     }
-    __device__ __forceinline__ int page_of(int i) const { return ALIGNED ? page : __shfl_sync(0xffffffffu, page, i); }
-    __device__ __forceinline__ unsigned slot_of(int i) const { return ALIGNED ? slot + i : __shfl_sync(0xffffffffu, slot, i); }
 };
 
 // ------------------------------------------------------------------------------------------- 2- and 1-byte caches
-// One warp's share of a segment on the tensor cores: 16 tokens at a time.
+// One warp's share of a segment on the tensor cores, 16 or 32 tokens at a time.
 //
-// Lane (g, r) = (lane / 4, lane % 4).  Scores S = Q K^T: the lane's operand of K is 16 bytes of tokens g and 8 + g; it receives the
-// scores of head g with tokens 2r, 2r + 1, 8 + 2r, 9 + 2r.  Values O = P V: weights of just these tokens are its operand of P, and its
-// operand of V is 16 (or 8) bytes of the same four tokens, two tokens' values interleaved by byte permutes.
-template <int DTYPE, int DP>
+// Lane (g, r) = (lane / 4, lane % 4).  Scores S = Q K^T: the lane's operand of K is 16 bytes of tokens g and 8 + g of 16; it
+// receives the scores of head g with tokens 2r, 2r + 1, 8 + 2r, 9 + 2r.  Values O = P V: weights of just these tokens are its
+// operand of P, and its operand of V is 16 (or 8) bytes of the same four tokens, two tokens' values interleaved by byte permutes.
+template <int DTYPE, int DP, bool PACKED>
 struct TensorWarp {
-    static constexpr int HEADS = 8, TOKENS = 16;
+    static constexpr int HEADS = 8;
     static constexpr bool E4M3 = DTYPE == TE_KV_E4M3;
     static constexpr int ES = E4M3 ? 1 : 2;
+    static constexpr int TOKENS = DP * ES <= 128 ? 32 : 16;             // 8 KB a stage (16 for bf16 rows of 256)
+    static constexpr int NK = TOKENS / 16;
+    typedef Ring<DP, ES, TOKENS, 3, E4M3, PACKED> R;
     static constexpr int KG = E4M3 ? DP / 64 : DP / 32;                 // groups of 4 lanes x 16 bytes of a key
-    static constexpr int KB = KG > 4 ? 4 : KG;                          // of which this many are in registers at a time
     static constexpr int VW = E4M3 && DP < 128 ? 8 : 16;                // bytes of a value a lane holds per chunk
     static constexpr int VE = VW / ES;                                  // elements of it
     static constexpr int VC = DP / (8 * VE);                            // chunks of 8 lanes
-    static constexpr int VB = VC > 2 ? 2 : VC;
     static constexpr int QWORDS = E4M3 ? 16 : 12;                       // 32-bit words of query terms per (group, lane)
     static constexpr int Q_BYTES = KG * 32 * QWORDS * 4;
+    static constexpr int MIN_BLOCKS = R::BYTES * WARPS > 110000 ? 1 : 2;
     static constexpr float LIFT = 10.0f;        // e4m3: weights reach 2^10, so that the lower of their two half terms keeps 2^-34 of the largest
 
     // Splits the tile's queries into terms, in the order the tensor operand wants them.  q_unit: e4m3 only, what the scores of a head
@@ -215,115 +339,81 @@ struct TensorWarp {
         }
     }
 
-    float acc[VC * VE][4];     // [n tile][row g: 2 columns, row g + 8: 2 columns]
+    float acc[VC * VE][2];     // [n tile][2 columns] of head g, both rows of its terms
     float m, l;                // of head g; l over this lane's tokens only
     float mv;                  // e4m3: the maximum the values' weights are measured against
 
-    template <bool ALIGNED>
-    __device__ void run(const AttnParams& p, const Segment& s, const unsigned* words, const float* q_unit, int64_t tile, int64_t tile_end) {
+    // The tensor core truncates as it adds to its accumulator, which over many tokens would shrink the sums; so each 16 tokens'
+    // product starts from zero and is added here, rounded to nearest, with the rescaling in the same FMA.
+    __device__ __forceinline__ void add(int i, const float (&x)[4], float keep) {
+        acc[i][0] = fmaf(acc[i][0], keep, x[0] + x[2]);
+        acc[i][1] = fmaf(acc[i][1], keep, x[1] + x[3]);
+    }
+
+    __device__ void run(const AttnParams& p, const Segment& s, const unsigned* words, const float* q_unit, char* ring, int64_t tile, int64_t tile_end) {
         const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, r = lane % 4;
         const int64_t* table = p.page_table + s.row * p.table_stride;
         const RowRange range = s.range;
-        constexpr int64_t STEP = WARPS * TOKENS;
-        int64_t t0 = tile * STEP + warp * TOKENS;
-        const int64_t t_end = tile_end * STEP;
+        int64_t t0 = tile * R::STEP + warp * TOKENS;               // of the stage to be issued
+        const int64_t t_end = tile_end * R::STEP;
+        const int stages = (int)((tile_end - tile));               // every warp has one stage of each tile
 #pragma unroll
-        for (int i = 0; i < VC * VE; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+        for (int i = 0; i < VC * VE; ++i) acc[i][0] = acc[i][1] = 0.0f;
         m = mv = -INFINITY;
         l = 0.0f;
-        const char* kbase = p.kc + s.kv_head * p.kcs[1] + r * 16;
-        const char* vbase = p.vc + s.kv_head * p.vcs[1] + g * VW;
         const float unit = p.scale * LOG2E * (E4M3 ? q_unit[g] : 1.0f);
-        Places<ALIGNED, TOKENS> here, next;
-        uint4 k[2][KB];
-        uint4 v[4][VB];
-        float ks[4], vs[4];
-        auto token = [&](int i) { return i < 2 ? 2 * r + i : 6 + 2 * r + i; };     // the four tokens whose scores this lane holds
-        auto load_k = [&](const Places<ALIGNED, TOKENS>& at, int64_t base, int batch) {
+        R copies;
+        copies.base = smem_address(ring);
+        unsigned seen[R::STAGES];
+        copies.look_up(p, table, t0, t_end, range.n);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int page = at.page_of(g + 8 * i);
-                const unsigned slot = at.slot_of(g + 8 * i);
-                const int64_t t = base + g + 8 * i;
-                const bool in = page >= 0 && t >= range.first && t < range.n;
-                const char* row = kbase + page * p.kcs[0] + slot * p.kcs[2];
-#pragma unroll
-                for (int c = 0; c < KB; ++c) {
-                    const int byte = (batch * KB + c) * 64;
-                    k[i][c] = load16(row + byte, in && byte + r * 16 < p.d * ES);
-                }
+        for (int i = 0; i < R::STAGES - 1; ++i) {
+            seen[i] = 0u;
+            if (i < stages) {
+                seen[i] = copies.issue(p, range, s.kv_head, t0, i);
+                t0 += R::STEP;
+                copies.look_up(p, table, t0, t_end, range.n);
             }
-        };
-        auto load_v = [&](const Places<ALIGNED, TOKENS>& at, int64_t base, int batch) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int page = at.page_of(token(i));
-                const unsigned slot = at.slot_of(token(i));
-                const int64_t t = base + token(i);
-                const bool in = page >= 0 && t >= range.first && t < range.n;
-                const char* row = vbase + page * p.vcs[0] + slot * p.vcs[2];
-#pragma unroll
-                for (int c = 0; c < VB; ++c) {
-                    const int byte = (batch * VB + c) * 8 * VW;
-                    const bool wanted = in && byte + g * VW < p.d * ES;
-                    if constexpr (VW == 16) {
-                        v[i][c] = load16(row + byte, wanted);
-                    } else {
-                        uint2 w = make_uint2(0u, 0u);
-                        if (wanted) w = __ldg(reinterpret_cast<const uint2*>(row + byte));
-                        v[i][c] = make_uint4(w.x, w.y, 0u, 0u);
-                    }
-                }
-            }
-        };
-        auto load_scales = [&](const Places<ALIGNED, TOKENS>& at, int64_t base) {
-            if constexpr (E4M3) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int page = at.page_of(token(i));
-                    const unsigned slot = at.slot_of(token(i));
-                    const int64_t t = base + token(i);
-                    const bool in = page >= 0 && t >= range.first && t < range.n;
-                    const int64_t o = page * p.ss[0] + s.kv_head * p.ss[1] + slot * p.ss[2];
-                    ks[i] = in ? __ldg(p.k_scale + o) : 1.0f;
-                    vs[i] = in ? __ldg(p.v_scale + o) : 1.0f;
-                }
-            }
-        };
-        if (t0 < t_end) {
-            here.fetch(p, table, t0, lane, range.n);
-            next.fetch(p, table, t0 + STEP, lane, range.n);
-            here.settle(p, t0, lane, range);
-            load_k(here, t0, 0);
-            load_scales(here, t0);
-            load_v(here, t0, 0);
+            copies_issued();
         }
-        for (; t0 < t_end; t0 += STEP) {
-            const int64_t t1 = t0 + STEP;
-            const bool more = t1 < t_end;
+        int at = 0, to = R::STAGES - 1;
+        for (int n = 0; n < stages; ++n) {
+            copies_wait<R::STAGES - 2>();
+            __syncwarp();                  // this stage has landed for all lanes, and all are done with the one before it
+            if (t0 < t_end) {
+                seen[R::STAGES - 1] = copies.issue(p, range, s.kv_head, t0, to);
+                t0 += R::STEP;
+                copies.look_up(p, table, t0, t_end, range.n);
+            }
+            copies_issued();
+            const char* keys = copies.stage(ring, at);
+            const char* values = keys + R::SIDE;
+            const float* scales = reinterpret_cast<const float*>(keys + 2 * R::SIDE);
             // ---- scores
-            float sc[2][4] = {};
+            float w[NK][4], vs[NK][4];
+            float top = -INFINITY, topv = -INFINITY;
 #pragma unroll
-            for (int b = 0; b < KG / KB; ++b) {
+            for (int nk = 0; nk < NK; ++nk) {
+                float sc[2][4] = {};
 #pragma unroll
-                for (int c = 0; c < KB; ++c) {
+                for (int c = 0; c < KG; ++c) {
                     constexpr int QUARTER = KG * 32 * 4;
-                    const uint4* w = reinterpret_cast<const uint4*>(words + ((b * KB + c) * 32 + lane) * 4);
+                    const uint4* q = reinterpret_cast<const uint4*>(words + (c * 32 + lane) * 4);
                     if constexpr (E4M3) {
-                        const uint4 h0 = w[0], h1 = w[QUARTER / 4], l0 = w[2 * QUARTER / 4], l1 = w[3 * QUARTER / 4];
+                        const uint4 h0 = q[0], h1 = q[QUARTER / 4], l0 = q[2 * QUARTER / 4], l1 = q[3 * QUARTER / 4];
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const uint4 x = k[i][c];
+                            const uint4 x = *reinterpret_cast<const uint4*>(keys + R::key_at(nk * 16 + i * 8 + g, 4 * c + r));
                             mma_f16(sc[i], h0.x, l0.x, h0.y, l0.y, half_of_e4m3(x.x), half_of_e4m3(x.x >> 16));
                             mma_f16(sc[i], h0.z, l0.z, h0.w, l0.w, half_of_e4m3(x.y), half_of_e4m3(x.y >> 16));
                             mma_f16(sc[i], h1.x, l1.x, h1.y, l1.y, half_of_e4m3(x.z), half_of_e4m3(x.z >> 16));
                             mma_f16(sc[i], h1.z, l1.z, h1.w, l1.w, half_of_e4m3(x.w), half_of_e4m3(x.w >> 16));
                         }
                     } else {
-                        const uint4 hi = w[0], mid = w[QUARTER / 4], lo = w[2 * QUARTER / 4];
+                        const uint4 hi = q[0], mid = q[QUARTER / 4], lo = q[2 * QUARTER / 4];
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const uint4 x = k[i][c];
+                            const uint4 x = *reinterpret_cast<const uint4*>(keys + R::key_at(nk * 16 + i * 8 + g, 4 * c + r));
                             mma_bf16(sc[i], hi.x, mid.x, hi.y, mid.y, x.x, x.y);
                             mma_bf16(sc[i], lo.x, 0u, lo.y, 0u, x.x, x.y);
                             mma_bf16(sc[i], hi.z, mid.z, hi.w, mid.w, x.z, x.w);
@@ -331,47 +421,34 @@ struct TensorWarp {
                         }
                     }
                 }
-                if (b + 1 < KG / KB) load_k(here, t0, b + 1);
-            }
-            // ---- the next tokens' keys
-            if (more) {
-                next.settle(p, t1, lane, range);
-                load_k(next, t1, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = nk * 16 + 8 * (i / 2) + 2 * r + i % 2;
+                    float x = (sc[i / 2][i % 2] + sc[i / 2][2 + i % 2]) * unit;
+                    if constexpr (E4M3) x *= scales[t];
+                    w[nk][i] = seen[0] >> t & 1u ? x : -INFINITY;
+                    top = fmaxf(top, w[nk][i]);
+                    if constexpr (E4M3) {       // a value's scale goes into its weight: 2^e, e from the exponent field
+                        vs[nk][i] = w[nk][i] + (float)((int)(__float_as_uint(scales[TOKENS + t]) >> 23) - 127);
+                        topv = fmaxf(topv, vs[nk][i]);
+                    }
+                }
             }
             // ---- weights
-            float w[4], top = -INFINITY, topv = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int64_t t = t0 + token(i);
-                const int page = here.page_of(token(i));          // (all lanes take part)
-                const bool seen = page >= 0 && t >= range.first && t < range.n;
-                float x = (sc[i / 2][i % 2] + sc[i / 2][2 + i % 2]) * unit;
-                if constexpr (E4M3) x *= ks[i];
-                w[i] = seen ? x : -INFINITY;
-                top = fmaxf(top, w[i]);
-            }
-            float sum = 0.0f;
-            if constexpr (E4M3) {
-                // the values' scales go into their weights: 2^e, e from the exponent field
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vs[i] = w[i] + (float)((int)(__float_as_uint(vs[i]) >> 23) - 127);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) topv = fmaxf(topv, vs[i]);
-            }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             top = fmaxf(top, m);
             const float base = settled(top);
-            float keep = exp2f(m - base);
-            l *= keep;
+            float keep = exp2f(m - base), sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float e = exp2f(w[i] - base);
-                sum += e;
-                if constexpr (!E4M3) w[i] = e;
-            }
-            l += sum;
-            bool moved = top != m;
+            for (int nk = 0; nk < NK; ++nk)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = exp2f(w[nk][i] - base);
+                    sum += e;
+                    if constexpr (!E4M3) w[nk][i] = e;
+                }
+            l = l * keep + sum;
             m = top;
             if constexpr (E4M3) {
                 topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 1));
@@ -380,79 +457,86 @@ struct TensorWarp {
                 const float basev = settled(topv);
                 keep = exp2f(mv - basev);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = exp2f(vs[i] - basev + LIFT);
-                moved = topv != mv;
+                for (int nk = 0; nk < NK; ++nk)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[nk][i] = exp2f(vs[nk][i] - basev + LIFT);
                 mv = topv;
-                if (more) load_scales(next, t1);
             }
-            if (__any_sync(0xffffffffu, moved)) {
+            unsigned a[NK][6];
 #pragma unroll
-                for (int i = 0; i < VC * VE; ++i) {
-                    acc[i][0] *= keep; acc[i][1] *= keep; acc[i][2] *= keep; acc[i][3] *= keep;
-                }
-            }
-            unsigned a[6];
-            if constexpr (E4M3) {
+            for (int nk = 0; nk < NK; ++nk)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    a[i] = pack_half(w[2 * i], w[2 * i + 1]);
-                    const float2 f = unpack_half(a[i]);
-                    a[2 + i] = pack_half(w[2 * i] - f.x, w[2 * i + 1] - f.y);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float x = w[2 * i], y = w[2 * i + 1];
-                    a[i] = pack_bf16(x, y);
-                    x -= bf16_lo(a[i]);
-                    y -= bf16_hi(a[i]);
-                    a[2 + i] = pack_bf16(x, y);
-                    a[4 + i] = pack_bf16(x - bf16_lo(a[2 + i]), y - bf16_hi(a[2 + i]));
-                }
-            }
-            // ---- values
-#pragma unroll
-            for (int b = 0; b < VC / VB; ++b) {
-#pragma unroll
-                for (int c = 0; c < VB; ++c) {
-                    const int n0 = (b * VB + c) * VE;
-                    const unsigned x[4][4] = {{v[0][c].x, v[0][c].y, v[0][c].z, v[0][c].w}, {v[1][c].x, v[1][c].y, v[1][c].z, v[1][c].w},
-                                              {v[2][c].x, v[2][c].y, v[2][c].z, v[2][c].w}, {v[3][c].x, v[3][c].y, v[3][c].z, v[3][c].w}};
-#pragma unroll
-                    for (int i = 0; i < VW / 4; ++i) {
-                        if constexpr (E4M3) {
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const unsigned y0 = __byte_perm(x[0][i], x[1][i], e ? 0x7362 : 0x5140), y1 = __byte_perm(x[2][i], x[3][i], e ? 0x7362 : 0x5140);
-                                mma_f16(acc[n0 + 4 * i + 2 * e], a[0], a[2], a[1], a[3], half_of_e4m3(y0), half_of_e4m3(y1));
-                                mma_f16(acc[n0 + 4 * i + 2 * e + 1], a[0], a[2], a[1], a[3], half_of_e4m3(y0 >> 16), half_of_e4m3(y1 >> 16));
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const unsigned y0 = __byte_perm(x[0][i], x[1][i], e ? 0x7632 : 0x5410), y1 = __byte_perm(x[2][i], x[3][i], e ? 0x7632 : 0x5410);
-                                mma_bf16(acc[n0 + 2 * i + e], a[0], a[2], a[1], a[3], y0, y1);
-                                mma_bf16(acc[n0 + 2 * i + e], a[4], 0u, a[5], 0u, y0, y1);
-                            }
-                        }
+                    float x = w[nk][2 * i], y = w[nk][2 * i + 1];
+                    if constexpr (E4M3) {
+                        a[nk][i] = pack_half(x, y);
+                        const float2 f = unpack_half(a[nk][i]);
+                        a[nk][2 + i] = pack_half(x - f.x, y - f.y);
+                    } else {
+                        a[nk][i] = pack_bf16(x, y);
+                        x -= bf16_lo(a[nk][i]);
+                        y -= bf16_hi(a[nk][i]);
+                        a[nk][2 + i] = pack_bf16(x, y);
+                        a[nk][4 + i] = pack_bf16(x - bf16_lo(a[nk][2 + i]), y - bf16_hi(a[nk][2 + i]));
                     }
                 }
-                if (b + 1 < VC / VB) load_v(here, t0, b + 1);
+            // ---- values
+#pragma unroll
+            for (int c = 0; c < VC; ++c) {
+                unsigned x[NK][4][4];
+#pragma unroll
+                for (int nk = 0; nk < NK; ++nk)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int t = nk * 16 + 8 * (i / 2) + 2 * r + i % 2;
+                        if constexpr (VW == 16) {
+                            const uint4 v = *reinterpret_cast<const uint4*>(values + R::value_at(t, 8 * c + g));
+                            x[nk][i][0] = v.x; x[nk][i][1] = v.y; x[nk][i][2] = v.z; x[nk][i][3] = v.w;
+                        } else {
+                            const uint2 v = *reinterpret_cast<const uint2*>(values + R::value_at(t, 4 * c + g / 2) + g % 2 * 8);
+                            x[nk][i][0] = v.x; x[nk][i][1] = v.y;
+                        }
+                    }
+#pragma unroll
+                for (int i = 0; i < VW / 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float y0[4] = {}, y1[4] = {};
+#pragma unroll
+                        for (int nk = 0; nk < NK; ++nk) {
+                            if constexpr (E4M3) {
+                                const unsigned b0 = __byte_perm(x[nk][0][i], x[nk][1][i], e ? 0x7362 : 0x5140), b1 = __byte_perm(x[nk][2][i], x[nk][3][i], e ? 0x7362 : 0x5140);
+                                mma_f16(y0, a[nk][0], a[nk][2], a[nk][1], a[nk][3], half_of_e4m3(b0), half_of_e4m3(b1));
+                                mma_f16(y1, a[nk][0], a[nk][2], a[nk][1], a[nk][3], half_of_e4m3(b0 >> 16), half_of_e4m3(b1 >> 16));
+                            } else {
+                                const unsigned b0 = __byte_perm(x[nk][0][i], x[nk][1][i], e ? 0x7632 : 0x5410), b1 = __byte_perm(x[nk][2][i], x[nk][3][i], e ? 0x7632 : 0x5410);
+                                mma_bf16(y0, a[nk][0], a[nk][2], a[nk][1], a[nk][3], b0, b1);
+                                mma_bf16(y0, a[nk][4], 0u, a[nk][5], 0u, b0, b1);
+                            }
+                        }
+                        if constexpr (E4M3) {
+                            add(c * VE + 4 * i + 2 * e, y0, keep);
+                            add(c * VE + 4 * i + 2 * e + 1, y1, keep);
+                        } else {
+                            add(c * VE + 2 * i + e, y0, keep);
+                        }
+                    }
             }
-            if (more) {
-                load_v(next, t1, 0);
-                here = next;
-                next.fetch(p, table, t1 + STEP, lane, range.n);
-            }
+#pragma unroll
+            for (int i = 0; i + 1 < R::STAGES; ++i) seen[i] = seen[i + 1];
+            at = at + 1 == R::STAGES ? 0 : at + 1;
+            to = to + 1 == R::STAGES ? 0 : to + 1;
         }
+        copies_wait<0>();
+        __syncwarp();                      // the ring is free for the sums
         // one sum per head, and e4m3 sums measured against m like the others
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         const float back = E4M3 ? exp2f(settled(mv) - settled(m) - LIFT) : 1.0f;
 #pragma unroll
         for (int i = 0; i < VC * VE; ++i) {
-            acc[i][0] = (acc[i][0] + acc[i][2]) * back;
-            acc[i][1] = (acc[i][1] + acc[i][3]) * back;
+            acc[i][0] *= back;
+            acc[i][1] *= back;
         }
     }
 
@@ -472,22 +556,24 @@ struct TensorWarp {
 };
 
 // ------------------------------------------------------------------------------------------------------ FP32 cache
-// One warp's share of a segment with FP32 FMAs, HT heads at once.  Scores: lane (g, r) holds 16-byte pieces r, r + 4, .. of
+// One warp's share of a segment with FP32 FMAs, HT heads at once.  Scores: lane (g, r) takes 16-byte pieces r, r + 4, .. of
 // token g's key (and of token 8 + g's), and four lanes add up to a score.  Values: the lanes lie along d, and the weights
 // come back through a few words of shared memory.
-template <int DP, int HT>
+template <int DP, int HT, bool PACKED>
 struct FmaWarp {
     static constexpr int HEADS = HT;
     static constexpr int TOKENS = DP <= 64 ? 16 : 8;
-    static constexpr int TG = TOKENS / 8;                  // tokens whose keys a lane holds parts of
-    static constexpr int KC = DP / 16;                     // 16-byte pieces of a key a lane holds
+    typedef Ring<DP, 4, TOKENS, 3, false, PACKED> R;
+    static constexpr int TG = TOKENS / 8;                  // tokens whose keys a lane takes parts of
+    static constexpr int KC = DP / 16;                     // 16-byte pieces of a key a lane takes
     static constexpr int LPT = DP / 4 < 32 ? DP / 4 : 32;  // lanes along a value
-    static constexpr int TPI = 32 / LPT;                   // tokens per load instruction
-    static constexpr int VC = DP / 4 / LPT;                // pieces of a value a lane holds
+    static constexpr int TPI = 32 / LPT;                   // tokens the warp takes at once
+    static constexpr int VC = DP / 4 / LPT;                // pieces of a value a lane takes
     static constexpr int VI = TOKENS / TPI;
     static constexpr int OWN = (HT + 3) / 4;               // heads whose weights a lane computes
-    static constexpr int Q_BYTES = HT * DP * 4;
-    static constexpr int W_BYTES = (TOKENS * HT + HT) * 8; // per warp: weights and factors, doubled for two FMAs at once
+    static constexpr int Q_BYTES = HT * DP * 4 + WARPS * (TOKENS * HT + HT) * 8;     // queries, then each warp's weights and factors,
+                                                                                     // doubled for two FMAs at once
+    static constexpr int MIN_BLOCKS = R::BYTES * WARPS > 110000 ? 1 : 2;
 
     static __device__ void stage_queries(const AttnParams& p, const Segment& s, float* words) {
         const float* q = p.q + s.row * p.qs[0] + s.head0 * p.qs[1];
@@ -500,14 +586,14 @@ struct FmaWarp {
     unsigned long long acc[HT][VC][2];
     float m[OWN], l[OWN];          // of heads r, r + 4 (modulo HT); l over this lane's tokens only
 
-    template <bool ALIGNED>
-    __device__ void run(const AttnParams& p, const Segment& s, const float* q, unsigned long long* weights, int64_t tile, int64_t tile_end) {
+    __device__ void run(const AttnParams& p, const Segment& s, const float* q, char* ring, int64_t tile, int64_t tile_end) {
         const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, r = lane % 4;
         const int64_t* table = p.page_table + s.row * p.table_stride;
         const RowRange range = s.range;
-        constexpr int64_t STEP = WARPS * TOKENS;
-        int64_t t0 = tile * STEP + warp * TOKENS;
-        const int64_t t_end = tile_end * STEP;
+        int64_t t0 = tile * R::STEP + warp * TOKENS;               // of the stage to be issued
+        const int64_t t_end = tile_end * R::STEP;
+        const int stages = (int)(tile_end - tile);                 // every warp has one stage of each tile
+        unsigned long long* weights = reinterpret_cast<unsigned long long*>(const_cast<float*>(q) + HT * DP) + warp * (TOKENS * HT + HT);
         unsigned long long* factors = weights + TOKENS * HT;
 #pragma unroll
         for (int h = 0; h < HT; ++h)
@@ -515,82 +601,59 @@ struct FmaWarp {
             for (int c = 0; c < VC; ++c) acc[h][c][0] = acc[h][c][1] = 0ull;
 #pragma unroll
         for (int i = 0; i < OWN; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
-        const char* kbase = p.kc + s.kv_head * p.kcs[1] + r * 16;
         const int along = lane % LPT, which = lane / LPT;
-        const char* vbase = p.vc + s.kv_head * p.vcs[1] + along * 16;
         const float unit = p.scale * LOG2E;
-        Places<ALIGNED, TOKENS> here, next;
-        uint4 k[TG][KC];
-        uint4 v[VI][VC];
-        auto load_k = [&](const Places<ALIGNED, TOKENS>& at, int64_t base) {
+        R copies;
+        copies.base = smem_address(ring);
+        unsigned seen[R::STAGES];
+        copies.look_up(p, table, t0, t_end, range.n);
 #pragma unroll
-            for (int i = 0; i < TG; ++i) {
-                const int page = at.page_of(g + 8 * i);
-                const unsigned slot = at.slot_of(g + 8 * i);
-                const int64_t t = base + g + 8 * i;
-                const bool in = page >= 0 && t >= range.first && t < range.n;
-                const char* row = kbase + page * p.kcs[0] + slot * p.kcs[2];
-#pragma unroll
-                for (int c = 0; c < KC; ++c) k[i][c] = load16(row + c * 64, in && c * 64 + r * 16 < p.d * 4);
+        for (int i = 0; i < R::STAGES - 1; ++i) {
+            seen[i] = 0u;
+            if (i < stages) {
+                seen[i] = copies.issue(p, range, s.kv_head, t0, i);
+                t0 += R::STEP;
+                copies.look_up(p, table, t0, t_end, range.n);
             }
-        };
-        auto load_v = [&](const Places<ALIGNED, TOKENS>& at, int64_t base) {
-#pragma unroll
-            for (int i = 0; i < VI; ++i) {
-                const int tk = i * TPI + which;
-                const int page = at.page_of(tk);
-                const unsigned slot = at.slot_of(tk);
-                const int64_t t = base + tk;
-                const bool in = page >= 0 && t >= range.first && t < range.n;
-                const char* row = vbase + page * p.vcs[0] + slot * p.vcs[2];
-#pragma unroll
-                for (int c = 0; c < VC; ++c) v[i][c] = load16(row + c * 512, in && c * 512 + along * 16 < p.d * 4);
-            }
-        };
-        if (t0 < t_end) {
-            here.fetch(p, table, t0, lane, range.n);
-            next.fetch(p, table, t0 + STEP, lane, range.n);
-            here.settle(p, t0, lane, range);
-            load_k(here, t0);
-            load_v(here, t0);
+            copies_issued();
         }
-        for (; t0 < t_end; t0 += STEP) {
-            const int64_t t1 = t0 + STEP;
-            const bool more = t1 < t_end;
+        int at = 0, to = R::STAGES - 1;
+        for (int n = 0; n < stages; ++n) {
+            copies_wait<R::STAGES - 2>();
+            __syncwarp();                  // this stage has landed for all lanes, and all are done with the one before it
+            if (t0 < t_end) {
+                seen[R::STAGES - 1] = copies.issue(p, range, s.kv_head, t0, to);
+                t0 += R::STEP;
+                copies.look_up(p, table, t0, t_end, range.n);
+            }
+            copies_issued();
+            const char* keys = copies.stage(ring, at);
+            const char* values = keys + R::SIDE;
             // ---- scores: every lane of a quad ends with the sums of all heads
             float sc[TG][HT];
 #pragma unroll
-            for (int h = 0; h < HT; ++h) {
-                unsigned long long part[TG][2];
+            for (int i = 0; i < TG; ++i) {
+                unsigned long long part[HT][2];
 #pragma unroll
-                for (int i = 0; i < TG; ++i) part[i][0] = part[i][1] = 0ull;
+                for (int h = 0; h < HT; ++h) part[h][0] = part[h][1] = 0ull;
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {
-                    const ulonglong2 qq = *reinterpret_cast<const ulonglong2*>(q + h * DP + c * 16 + r * 4);
+                    const ulonglong2 kk = *reinterpret_cast<const ulonglong2*>(keys + R::key_at(g + 8 * i, 4 * c + r));
 #pragma unroll
-                    for (int i = 0; i < TG; ++i) {
-                        const ulonglong2 kk = *reinterpret_cast<const ulonglong2*>(&k[i][c]);
-                        fma2(part[i][0], qq.x, kk.x);
-                        fma2(part[i][1], qq.y, kk.y);
+                    for (int h = 0; h < HT; ++h) {
+                        const ulonglong2 qq = *reinterpret_cast<const ulonglong2*>(q + h * DP + c * 16 + r * 4);
+                        fma2(part[h][0], qq.x, kk.x);
+                        fma2(part[h][1], qq.y, kk.y);
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < TG; ++i) {
-                    const float2 x = unpair(part[i][0]), y = unpair(part[i][1]);
-                    sc[i][h] = (x.x + x.y) + (y.x + y.y);
-                }
-            }
-            if (more) {
-                next.settle(p, t1, lane, range);
-                load_k(next, t1);
-            }
-#pragma unroll
-            for (int i = 0; i < TG; ++i)
-#pragma unroll
                 for (int h = 0; h < HT; ++h) {
+                    const float2 x = unpair(part[h][0]), y = unpair(part[h][1]);
+                    sc[i][h] = (x.x + x.y) + (y.x + y.y);
                     sc[i][h] += __shfl_xor_sync(0xffffffffu, sc[i][h], 1);
                     sc[i][h] += __shfl_xor_sync(0xffffffffu, sc[i][h], 2);
                 }
+            }
             // ---- weights of heads r, r + 4 over tokens g (and 8 + g)
             bool moved = false;
 #pragma unroll
@@ -602,10 +665,7 @@ struct FmaWarp {
                     float x = sc[i][(4 * j) % HT];
 #pragma unroll
                     for (int u = 1; u < 4; ++u) x = r == u ? sc[i][(u + 4 * j) % HT] : x;
-                    const int64_t t = t0 + g + 8 * i;
-                    const int page = here.page_of(g + 8 * i);      // (all lanes take part)
-                    const bool seen = page >= 0 && t >= range.first && t < range.n;
-                    w[i] = seen ? x * unit : -INFINITY;
+                    w[i] = seen[0] >> (g + 8 * i) & 1u ? x * unit : -INFINITY;
                     top = fmaxf(top, w[i]);
                 }
 #pragma unroll
@@ -638,25 +698,26 @@ struct FmaWarp {
             // ---- values
 #pragma unroll
             for (int i = 0; i < VI; ++i) {
-                const unsigned long long* w = weights + (i * TPI + which) * HT;
+                const int t = i * TPI + which;
+                const unsigned long long* w = weights + t * HT;
 #pragma unroll
-                for (int h = 0; h < HT; ++h) {
-                    const unsigned long long x = w[h];
+                for (int c = 0; c < VC; ++c) {
+                    const ulonglong2 vv = *reinterpret_cast<const ulonglong2*>(values + R::value_at(t, c * 32 + along));
 #pragma unroll
-                    for (int c = 0; c < VC; ++c) {
-                        const ulonglong2 vv = *reinterpret_cast<const ulonglong2*>(&v[i][c]);
+                    for (int h = 0; h < HT; ++h) {
+                        const unsigned long long x = w[h];
                         fma2(acc[h][c][0], x, vv.x);
                         fma2(acc[h][c][1], x, vv.y);
                     }
                 }
             }
-            __syncwarp();
-            if (more) {
-                load_v(next, t1);
-                here = next;
-                next.fetch(p, table, t1 + STEP, lane, range.n);
-            }
+#pragma unroll
+            for (int i = 0; i + 1 < R::STAGES; ++i) seen[i] = seen[i + 1];
+            at = at + 1 == R::STAGES ? 0 : at + 1;
+            to = to + 1 == R::STAGES ? 0 : to + 1;
         }
+        copies_wait<0>();
+        __syncwarp();                      // the ring is free for the sums
 #pragma unroll
         for (int j = 0; j < OWN; ++j)
 #pragma unroll
@@ -694,17 +755,20 @@ struct FmaWarp {
     }
 };
 
-template <int DTYPE, int DP, int HT> struct WarpOf { typedef TensorWarp<DTYPE, DP> type; };
-template <int DP, int HT> struct WarpOf<TE_KV_F32, DP, HT> { typedef FmaWarp<DP, HT> type; };
+template <int DTYPE, int DP, int HT, bool PACKED> struct WarpOf { typedef TensorWarp<DTYPE, DP, PACKED> type; };
+template <int DP, int HT, bool PACKED> struct WarpOf<TE_KV_F32, DP, HT, PACKED> { typedef FmaWarp<DP, HT, PACKED> type; };
 
 // ---------------------------------------------------------------------------------------------------- the two kernels
-template <int DTYPE, int DP, int HT, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS, 2) paged_attention_kernel(const AttnParams p) {
-    typedef typename WarpOf<DTYPE, DP, HT>::type Warp;
-    constexpr int HEADS = Warp::HEADS, TILE = WARPS * Warp::TOKENS;
-    __shared__ __align__(16) char query[Warp::Q_BYTES];
-    // the warps' sums at a segment's end; FP32 weights while it runs
-    __shared__ __align__(16) float sums[WARPS][HEADS][DP];
+template <int DTYPE, int DP, int HT, bool PACKED>
+__global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::MIN_BLOCKS) paged_attention_kernel(const AttnParams p) {
+    typedef typename WarpOf<DTYPE, DP, HT, PACKED>::type Warp;
+    typedef typename Warp::R R;
+    constexpr int HEADS = Warp::HEADS, TILE = R::STEP;
+    extern __shared__ __align__(128) char shared[];
+    char* rings = shared;                                  // [WARPS][R::BYTES]; at a segment's end each warp's sums
+    char* query = shared + WARPS * R::BYTES;               // [Warp::Q_BYTES]
+    static_assert(HEADS * DP * 4 <= R::BYTES, "a warp's sums fit its ring");
+    auto sums = [&](int j, int h, int c) { return reinterpret_cast<float*>(rings + j * R::BYTES) + h * DP + c; };
     __shared__ float2 ml[WARPS][HEADS];
     __shared__ float q_unit[HEADS];
     __shared__ int64_t scan[WARPS];
@@ -797,19 +861,17 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention_kernel(const AttnP
         const int64_t tile0 = s.range.first / TILE + (unit - seg_begin), tile1 = s.range.first / TILE + (stop - seg_begin);
         {
             Warp mywarp;
+            char* ring = rings + warp * R::BYTES;
             if constexpr (DTYPE == TE_KV_F32) {
                 Warp::stage_queries(p, s, reinterpret_cast<float*>(query));
                 __syncthreads();
-                // the weights' words lie where this warp's own sums will go
-                static_assert(Warp::W_BYTES <= sizeof(sums[0]), "weights fit the warp's sums");
-                mywarp.template run<ALIGNED>(p, s, reinterpret_cast<const float*>(query), reinterpret_cast<unsigned long long*>(sums[warp]), tile0, tile1);
-                __syncwarp();
+                mywarp.run(p, s, reinterpret_cast<const float*>(query), ring, tile0, tile1);
             } else {
                 Warp::stage_queries(p, s, reinterpret_cast<unsigned*>(query), q_unit);
                 __syncthreads();
-                mywarp.template run<ALIGNED>(p, s, reinterpret_cast<const unsigned*>(query), q_unit, tile0, tile1);
+                mywarp.run(p, s, reinterpret_cast<const unsigned*>(query), q_unit, ring, tile0, tile1);
             }
-            mywarp.put(&sums[warp][0][0], ml[warp]);
+            mywarp.put(sums(warp, 0, 0), ml[warp]);
         }
         __syncthreads();
         // ---- the four warps' sums into the result, or into the workspace when the segment is shared with other workers
@@ -826,7 +888,7 @@ __global__ void __launch_bounds__(THREADS, 2) paged_attention_kernel(const AttnP
 #pragma unroll
             for (int j = 0; j < WARPS; ++j) {
                 const float f = exp2f(ml[j][h].x - base);
-                const float4 x = *reinterpret_cast<const float4*>(&sums[j][h][c]);
+                const float4 x = *reinterpret_cast<const float4*>(sums(j, h, c));
                 l += f * ml[j][h].y;
                 a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
             }
@@ -909,30 +971,44 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(const AttnP
 // of a tile is computed whether it is there or not.
 int heads_per_tile(int dtype, int64_t group) { return dtype != TE_KV_F32 ? 8 : group >= 5 ? 8 : group >= 3 ? 4 : (int)group; }
 
-// Thread blocks per SM: what the registers allow (two of 128 threads at up to 255 each).
-constexpr int BLOCKS_PER_SM = 2;
+// Thread blocks per SM: two where two rings fit the shared memory, one for the longest rows.
+int blocks_per_sm(int dtype, int64_t d) { return dtype == TE_KV_E4M3 || d <= 128 ? 2 : 1; }
 
 size_t workspace_need(const te_paged_attn_desc* t, int sm_count) {
     if (t->rows == 0 || t->q_heads == 0) return 0;
-    const size_t workers = (size_t)sm_count * BLOCKS_PER_SM, heads = heads_per_tile(t->cache.dtype, t->q_heads / t->cache.heads);
+    const size_t workers = (size_t)sm_count * blocks_per_sm(t->cache.dtype, t->cache.d), heads = heads_per_tile(t->cache.dtype, t->q_heads / t->cache.heads);
     return workers * 16 + 2 * workers * heads * (8 + 4 * (size_t)t->cache.d);
 }
 
+template <int DTYPE, int DP, int HT, bool PACKED>
+cudaError_t launch_form(te_b200_ctx* ctx, const AttnParams& p, int workers, cudaStream_t st) {
+    typedef typename WarpOf<DTYPE, DP, HT, PACKED>::type Warp;
+    auto kernel = paged_attention_kernel<DTYPE, DP, HT, PACKED>;
+    constexpr int bytes = WARPS * Warp::R::BYTES + Warp::Q_BYTES;
+    int& state = ctx->kernel_state[reinterpret_cast<const void*>(kernel)];
+    if (!state) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return e;
+        state = 1;
+    }
+    return launch_pdl(kernel, dim3(workers), dim3(THREADS), bytes, st, p);
+}
+
 template <int DTYPE, int DP, int HT>
-cudaError_t launch_tiles(const AttnParams& p, int workers, cudaStream_t st) {
-    const bool aligned = p.page_size.divisor % 16 == 0;       // a warp's 16 (or 8) tokens never straddle pages
-    return aligned ? launch_pdl(paged_attention_kernel<DTYPE, DP, HT, true>, dim3(workers), dim3(THREADS), 0, st, p)
-                   : launch_pdl(paged_attention_kernel<DTYPE, DP, HT, false>, dim3(workers), dim3(THREADS), 0, st, p);
+cudaError_t launch_tiles(te_b200_ctx* ctx, const AttnParams& p, int workers, cudaStream_t st) {
+    constexpr int64_t row = DP * (DTYPE == TE_KV_F32 ? 4 : DTYPE == TE_KV_BF16 ? 2 : 1);
+    const bool packed = p.d == DP && p.page_size.divisor % 16 == 0 && p.kcs[2] == row && p.vcs[2] == row;
+    return packed ? launch_form<DTYPE, DP, HT, true>(ctx, p, workers, st) : launch_form<DTYPE, DP, HT, false>(ctx, p, workers, st);
 }
 
 template <int DP>
-cudaError_t launch_width(const AttnParams& p, int dtype, int heads, int workers, cudaStream_t st) {
-    if (dtype == TE_KV_BF16) return launch_tiles<TE_KV_BF16, DP, 8>(p, workers, st);
-    if (dtype == TE_KV_E4M3) return launch_tiles<TE_KV_E4M3, DP, 8>(p, workers, st);
-    if (heads == 1) return launch_tiles<TE_KV_F32, DP, 1>(p, workers, st);
-    if (heads == 2) return launch_tiles<TE_KV_F32, DP, 2>(p, workers, st);
-    if (heads == 4) return launch_tiles<TE_KV_F32, DP, 4>(p, workers, st);
-    return launch_tiles<TE_KV_F32, DP, 8>(p, workers, st);
+cudaError_t launch_width(te_b200_ctx* ctx, const AttnParams& p, int dtype, int heads, int workers, cudaStream_t st) {
+    if (dtype == TE_KV_BF16) return launch_tiles<TE_KV_BF16, DP, 8>(ctx, p, workers, st);
+    if (dtype == TE_KV_E4M3) return launch_tiles<TE_KV_E4M3, DP, 8>(ctx, p, workers, st);
+    if (heads == 1) return launch_tiles<TE_KV_F32, DP, 1>(ctx, p, workers, st);
+    if (heads == 2) return launch_tiles<TE_KV_F32, DP, 2>(ctx, p, workers, st);
+    if (heads == 4) return launch_tiles<TE_KV_F32, DP, 4>(ctx, p, workers, st);
+    return launch_tiles<TE_KV_F32, DP, 8>(ctx, p, workers, st);
 }
 
 int check_desc(const te_paged_attn_desc* t) {
@@ -980,7 +1056,7 @@ int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* t, te_st
         snprintf(msg, sizeof msg, "context workspace (%zu bytes) too small; paged attention needs %zu bytes", ctx->workspace_bytes, need);
         return fail(TE_ERR_WORKSPACE, msg);
     }
-    const int workers = ctx->sm_count * BLOCKS_PER_SM;
+    const int workers = ctx->sm_count * blocks_per_sm(c.dtype, c.d);
     AttnParams p;
     p.q = t->q; p.o = t->o; p.lse = t->lse;
     p.kc = static_cast<const char*>(c.k); p.vc = static_cast<const char*>(c.v); p.k_scale = c.k_scale; p.v_scale = c.v_scale;
@@ -1001,8 +1077,8 @@ int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* t, te_st
     p.part_acc = reinterpret_cast<float*>(ws + (size_t)workers * 16 + (size_t)workers * 2 * heads * 8);
     p.status = ctx->d_status;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e = p.d <= 64 ? launch_width<64>(p, c.dtype, heads, workers, st) : p.d <= 128 ? launch_width<128>(p, c.dtype, heads, workers, st)
-                                                                                  : launch_width<256>(p, c.dtype, heads, workers, st);
+    cudaError_t e = p.d <= 64 ? launch_width<64>(ctx, p, c.dtype, heads, workers, st) : p.d <= 128 ? launch_width<128>(ctx, p, c.dtype, heads, workers, st)
+                                                                                  : launch_width<256>(ctx, p, c.dtype, heads, workers, st);
     if (e != cudaSuccess) return cuda_fail(e, "paged_attention_kernel launch");
     e = launch_pdl(paged_join_kernel, dim3((unsigned)workers, (unsigned)heads), dim3(32 * JOIN_WARPS), 0, st, p, heads);
     if (e != cudaSuccess) return cuda_fail(e, "paged_join_kernel launch");
