@@ -65,13 +65,24 @@ struct Segment {
 };
 
 // ---------------------------------------------------------------------------------------------------- small pieces
-__device__ __forceinline__ void mma_bf16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// c += a b, and c = a b; a holds the four words of the left operand.
+template <bool HALF>
+__device__ __forceinline__ void mma(float (&c)[4], const uint4& a, unsigned b0, unsigned b1) {
+    if constexpr (HALF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_f16(float (&c)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+template <bool HALF>
+__device__ __forceinline__ void mma_from_zero(float (&c)[4], const uint4& a, unsigned b0, unsigned b1) {
+    if constexpr (HALF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -84,10 +95,10 @@ __device__ __forceinline__ unsigned pack_half(float lo, float hi) {
     return *reinterpret_cast<const unsigned*>(&v);
 }
 __device__ __forceinline__ float2 unpack_half(unsigned v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-// Two e4m3 values (low byte first) as two halves, exactly.
-__device__ __forceinline__ unsigned half_of_e4m3(unsigned two) {
-    unsigned r;
-    asm("{ .reg .b16 t; cvt.u16.u32 t, %1; cvt.rn.f16x2.e4m3x2 %0, t; }" : "=r"(r) : "r"(two));
+// Four e4m3 values (low byte first) as four halves, exactly.
+__device__ __forceinline__ uint2 halves_of_e4m3(unsigned four) {
+    uint2 r;
+    asm("{ .reg .b16 lo, hi; mov.b32 {lo, hi}, %2; cvt.rn.f16x2.e4m3x2 %0, lo; cvt.rn.f16x2.e4m3x2 %1, hi; }" : "=r"(r.x), "=r"(r.y) : "r"(four));
     return r;
 }
 __device__ __forceinline__ unsigned smem_address(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -283,8 +294,8 @@ struct TensorWarp {
     static constexpr int VW = E4M3 && DP < 128 ? 8 : 16;                // bytes of a value a lane holds per chunk
     static constexpr int VE = VW / ES;                                  // elements of it
     static constexpr int VC = DP / (8 * VE);                            // chunks of 8 lanes
-    static constexpr int QWORDS = E4M3 ? 16 : 12;                       // 32-bit words of query terms per (group, lane)
-    static constexpr int Q_BYTES = KG * 32 * QWORDS * 4;
+    static constexpr int KQ = 4;                                        // left operands of Q per group, 16 bytes a lane each
+    static constexpr int Q_BYTES = KG * KQ * 32 * 16;
     static constexpr int MIN_BLOCKS = R::BYTES * WARPS > 110000 ? 1 : 2;
     static constexpr float LIFT = 10.0f;        // e4m3: weights reach 2^10, so that the lower of their two half terms keeps 2^-34 of the largest
 
@@ -306,7 +317,9 @@ struct TensorWarp {
             }
             __syncthreads();
         }
-        // one thread per (group, lane, pair of elements)
+        // one thread per (group, lane, pair of elements); a left operand is {row g, row g + 8, row g, row g + 8} of pairs 2j, 2j, 2j + 1,
+        // 2j + 1.  e4m3: operand j of 4 holds upper and lower terms.  bf16: operand j of 2 upper and middle ones, operand 2 + j lower ones
+        // (and zeros in row g + 8).
         constexpr int PAIRS = E4M3 ? 8 : 4;
         for (int i = threadIdx.x; i < KG * 32 * PAIRS; i += THREADS) {
             const int j = i % PAIRS, lane = i / PAIRS % 32, c = i / PAIRS / 32;
@@ -317,24 +330,21 @@ struct TensorWarp {
                 x = q[g * p.qs[1] + at];
                 y = q[g * p.qs[1] + at + 1];
             }
-            unsigned* w = words + (c * 32 + lane) * 4;                 // [term quarter][group][lane][4]
-            constexpr int QUARTER = KG * 32 * 4;
+            unsigned* w = words + ((c * KQ + j / 2) * 32 + lane) * 4 + j % 2 * 2;
             if constexpr (E4M3) {
                 const float unit = 1.0f / q_unit[g];                   // a power of two
                 x *= unit;
                 y *= unit;
-                const unsigned hi = pack_half(x, y);
-                const float2 f = unpack_half(hi);
-                w[(j / 4) * QUARTER + j % 4] = hi;
-                w[(2 + j / 4) * QUARTER + j % 4] = pack_half(x - f.x, y - f.y);
+                w[0] = pack_half(x, y);
+                const float2 f = unpack_half(w[0]);
+                w[1] = pack_half(x - f.x, y - f.y);
             } else {
-                const unsigned hi = pack_bf16(x, y);
-                x -= bf16_lo(hi);
-                y -= bf16_hi(hi);
-                const unsigned mid = pack_bf16(x, y);
-                w[j] = hi;
-                w[QUARTER + j] = mid;
-                w[2 * QUARTER + j] = pack_bf16(x - bf16_lo(mid), y - bf16_hi(mid));
+                w[0] = pack_bf16(x, y);
+                x -= bf16_lo(w[0]);
+                y -= bf16_hi(w[0]);
+                w[1] = pack_bf16(x, y);
+                w[2 * 32 * 4] = pack_bf16(x - bf16_lo(w[1]), y - bf16_hi(w[1]));
+                w[2 * 32 * 4 + 1] = 0u;
             }
         }
     }
@@ -390,41 +400,39 @@ struct TensorWarp {
             const char* values = keys + R::SIDE;
             const float* scales = reinterpret_cast<const float*>(keys + 2 * R::SIDE);
             // ---- scores
+            float sc[NK][2][4];
+#pragma unroll
+            for (int c = 0; c < KG; ++c) {
+                const uint4* q = reinterpret_cast<const uint4*>(words) + c * KQ * 32 + lane;
+                const uint4 q0 = q[0], q1 = q[32], q2 = q[64], q3 = q[96];
+#pragma unroll
+                for (int i = 0; i < 2 * NK; ++i) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(keys + R::key_at(i * 8 + g, 4 * c + r));
+                    float (&y)[4] = sc[i / 2][i % 2];
+                    if constexpr (E4M3) {
+                        const uint2 k0 = halves_of_e4m3(x.x), k1 = halves_of_e4m3(x.y), k2 = halves_of_e4m3(x.z), k3 = halves_of_e4m3(x.w);
+                        if (c == 0) mma_from_zero<true>(y, q0, k0.x, k0.y);
+                        else mma<true>(y, q0, k0.x, k0.y);
+                        mma<true>(y, q1, k1.x, k1.y);
+                        mma<true>(y, q2, k2.x, k2.y);
+                        mma<true>(y, q3, k3.x, k3.y);
+                    } else {
+                        if (c == 0) mma_from_zero<false>(y, q0, x.x, x.y);
+                        else mma<false>(y, q0, x.x, x.y);
+                        mma<false>(y, q2, x.x, x.y);
+                        mma<false>(y, q1, x.z, x.w);
+                        mma<false>(y, q3, x.z, x.w);
+                    }
+                }
+            }
             float w[NK][4], vs[NK][4];
             float top = -INFINITY, topv = -INFINITY;
 #pragma unroll
-            for (int nk = 0; nk < NK; ++nk) {
-                float sc[2][4] = {};
-#pragma unroll
-                for (int c = 0; c < KG; ++c) {
-                    constexpr int QUARTER = KG * 32 * 4;
-                    const uint4* q = reinterpret_cast<const uint4*>(words + (c * 32 + lane) * 4);
-                    if constexpr (E4M3) {
-                        const uint4 h0 = q[0], h1 = q[QUARTER / 4], l0 = q[2 * QUARTER / 4], l1 = q[3 * QUARTER / 4];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(keys + R::key_at(nk * 16 + i * 8 + g, 4 * c + r));
-                            mma_f16(sc[i], h0.x, l0.x, h0.y, l0.y, half_of_e4m3(x.x), half_of_e4m3(x.x >> 16));
-                            mma_f16(sc[i], h0.z, l0.z, h0.w, l0.w, half_of_e4m3(x.y), half_of_e4m3(x.y >> 16));
-                            mma_f16(sc[i], h1.x, l1.x, h1.y, l1.y, half_of_e4m3(x.z), half_of_e4m3(x.z >> 16));
-                            mma_f16(sc[i], h1.z, l1.z, h1.w, l1.w, half_of_e4m3(x.w), half_of_e4m3(x.w >> 16));
-                        }
-                    } else {
-                        const uint4 hi = q[0], mid = q[QUARTER / 4], lo = q[2 * QUARTER / 4];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const uint4 x = *reinterpret_cast<const uint4*>(keys + R::key_at(nk * 16 + i * 8 + g, 4 * c + r));
-                            mma_bf16(sc[i], hi.x, mid.x, hi.y, mid.y, x.x, x.y);
-                            mma_bf16(sc[i], lo.x, 0u, lo.y, 0u, x.x, x.y);
-                            mma_bf16(sc[i], hi.z, mid.z, hi.w, mid.w, x.z, x.w);
-                            mma_bf16(sc[i], lo.z, 0u, lo.w, 0u, x.z, x.w);
-                        }
-                    }
-                }
+            for (int nk = 0; nk < NK; ++nk)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int t = nk * 16 + 8 * (i / 2) + 2 * r + i % 2;
-                    float x = (sc[i / 2][i % 2] + sc[i / 2][2 + i % 2]) * unit;
+                    float x = (sc[nk][i / 2][i % 2] + sc[nk][i / 2][2 + i % 2]) * unit;
                     if constexpr (E4M3) x *= scales[t];
                     w[nk][i] = seen[0] >> t & 1u ? x : -INFINITY;
                     top = fmaxf(top, w[nk][i]);
@@ -433,7 +441,6 @@ struct TensorWarp {
                         topv = fmaxf(topv, vs[nk][i]);
                     }
                 }
-            }
             // ---- weights
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -462,24 +469,25 @@ struct TensorWarp {
                     for (int i = 0; i < 4; ++i) w[nk][i] = exp2f(vs[nk][i] - basev + LIFT);
                 mv = topv;
             }
-            unsigned a[NK][6];
+            uint4 a[NK], lower[NK];         // left operands of P; bf16: the lowest terms apart
 #pragma unroll
-            for (int nk = 0; nk < NK; ++nk)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float x = w[nk][2 * i], y = w[nk][2 * i + 1];
-                    if constexpr (E4M3) {
-                        a[nk][i] = pack_half(x, y);
-                        const float2 f = unpack_half(a[nk][i]);
-                        a[nk][2 + i] = pack_half(x - f.x, y - f.y);
-                    } else {
-                        a[nk][i] = pack_bf16(x, y);
-                        x -= bf16_lo(a[nk][i]);
-                        y -= bf16_hi(a[nk][i]);
-                        a[nk][2 + i] = pack_bf16(x, y);
-                        a[nk][4 + i] = pack_bf16(x - bf16_lo(a[nk][2 + i]), y - bf16_hi(a[nk][2 + i]));
-                    }
+            for (int nk = 0; nk < NK; ++nk) {
+                float x0 = w[nk][0], x1 = w[nk][1], x2 = w[nk][2], x3 = w[nk][3];
+                if constexpr (E4M3) {
+                    a[nk].x = pack_half(x0, x1);
+                    a[nk].z = pack_half(x2, x3);
+                    const float2 f = unpack_half(a[nk].x), h = unpack_half(a[nk].z);
+                    a[nk].y = pack_half(x0 - f.x, x1 - f.y);
+                    a[nk].w = pack_half(x2 - h.x, x3 - h.y);
+                } else {
+                    a[nk].x = pack_bf16(x0, x1);
+                    a[nk].z = pack_bf16(x2, x3);
+                    x0 -= bf16_lo(a[nk].x); x1 -= bf16_hi(a[nk].x); x2 -= bf16_lo(a[nk].z); x3 -= bf16_hi(a[nk].z);
+                    a[nk].y = pack_bf16(x0, x1);
+                    a[nk].w = pack_bf16(x2, x3);
+                    lower[nk] = make_uint4(pack_bf16(x0 - bf16_lo(a[nk].y), x1 - bf16_hi(a[nk].y)), 0u, pack_bf16(x2 - bf16_lo(a[nk].w), x3 - bf16_hi(a[nk].w)), 0u);
                 }
+            }
             // ---- values
 #pragma unroll
             for (int c = 0; c < VC; ++c) {
@@ -501,17 +509,21 @@ struct TensorWarp {
                 for (int i = 0; i < VW / 4; ++i)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float y0[4] = {}, y1[4] = {};
+                        float y0[4], y1[4];
 #pragma unroll
                         for (int nk = 0; nk < NK; ++nk) {
                             if constexpr (E4M3) {
-                                const unsigned b0 = __byte_perm(x[nk][0][i], x[nk][1][i], e ? 0x7362 : 0x5140), b1 = __byte_perm(x[nk][2][i], x[nk][3][i], e ? 0x7362 : 0x5140);
-                                mma_f16(y0, a[nk][0], a[nk][2], a[nk][1], a[nk][3], half_of_e4m3(b0), half_of_e4m3(b1));
-                                mma_f16(y1, a[nk][0], a[nk][2], a[nk][1], a[nk][3], half_of_e4m3(b0 >> 16), half_of_e4m3(b1 >> 16));
+                                const uint2 b0 = halves_of_e4m3(__byte_perm(x[nk][0][i], x[nk][1][i], e ? 0x7362 : 0x5140));
+                                const uint2 b1 = halves_of_e4m3(__byte_perm(x[nk][2][i], x[nk][3][i], e ? 0x7362 : 0x5140));
+                                if (nk == 0) mma_from_zero<true>(y0, a[nk], b0.x, b1.x);
+                                else mma<true>(y0, a[nk], b0.x, b1.x);
+                                if (nk == 0) mma_from_zero<true>(y1, a[nk], b0.y, b1.y);
+                                else mma<true>(y1, a[nk], b0.y, b1.y);
                             } else {
                                 const unsigned b0 = __byte_perm(x[nk][0][i], x[nk][1][i], e ? 0x7632 : 0x5410), b1 = __byte_perm(x[nk][2][i], x[nk][3][i], e ? 0x7632 : 0x5410);
-                                mma_bf16(y0, a[nk][0], a[nk][2], a[nk][1], a[nk][3], b0, b1);
-                                mma_bf16(y0, a[nk][4], 0u, a[nk][5], 0u, b0, b1);
+                                if (nk == 0) mma_from_zero<false>(y0, a[nk], b0, b1);
+                                else mma<false>(y0, a[nk], b0, b1);
+                                mma<false>(y0, lower[nk], b0, b1);
                             }
                         }
                         if constexpr (E4M3) {
