@@ -23,6 +23,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "paged_plan.h"
 #include "pdl.cuh"
 #include "te_internal.h"
@@ -84,6 +86,11 @@ __device__ __forceinline__ void mma_from_zero(float (&c)[4], const uint4& a, uns
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.0f));
 }
+template <bool HALF>
+__device__ __forceinline__ void mma_first_or_next(bool first, float (&c)[4], const uint4& a, unsigned b0, unsigned b1) {
+    if (first) mma_from_zero<HALF>(c, a, b0, b1);
+    else mma<HALF>(c, a, b0, b1);
+}
 __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const unsigned*>(&v);
@@ -133,7 +140,13 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-// exp2 of a score less the maximum; a maximum of -infinity means that nothing has been seen.
+// 2^x to 2^-22 of itself, denormal results flushed: they are weights next to one of 1.
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// What is taken from a score before exp2_of: the maximum; one of -infinity means that nothing has been seen.
 __device__ __forceinline__ float settled(float m) { return m == -INFINITY ? 0.0f : m; }
 
 // A warp's ring: stages of TOKENS rows of keys and as many of values (and their scales), DP elements of ES bytes a row.
@@ -216,28 +229,32 @@ struct Ring {
             seen &= good;
         }
         if constexpr (PACKED) {
-            const bool all = seen == 0xffffffffu >> (32 - TOKENS);
+            const char *k[NB], *v[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const bool there = (good >> (b * BLOCK)) & 1u;
-                const char* k = kc + (there ? entry[b] * p.kcs[0] + slot[b] * (int64_t)RB : 0) + lane * 16;
-                const char* v = vc + (there ? entry[b] * p.vcs[0] + slot[b] * (int64_t)RB : 0) + lane * 16;
-#pragma unroll
-                for (int c = 0; c < BLOCK / TPI; ++c)
-#pragma unroll
-                    for (int u = 0; u < PPR; ++u) {
-                        const int t = b * BLOCK + c * TPI + sub;
-                        const unsigned kd = to + key_at(t, chunk + 32 * u), vd = to + SIDE + value_at(t, chunk + 32 * u);
-                        const int o = (c * PPR + u) * 512;
-                        if (all) {
-                            copy16(kd, k + o);
-                            copy16(vd, v + o);
-                        } else {
-                            copy16_or_zero(kd, k + o, seen >> t & 1u);
-                            copy16_or_zero(vd, v + o, seen >> t & 1u);
-                        }
-                    }
+                k[b] = kc + (there ? entry[b] * p.kcs[0] + slot[b] * (int64_t)RB : 0) + lane * 16;
+                v[b] = vc + (there ? entry[b] * p.vcs[0] + slot[b] * (int64_t)RB : 0) + lane * 16;
             }
+            auto copy = [&](auto whole) {
+#pragma unroll
+                for (int i = 0; i < TOKENS / TPI * PPR; ++i) {
+                    const int u = i % PPR, t = i / PPR * TPI + sub;                                     // (t: lane's token)
+                    constexpr int PER = BLOCK / TPI * PPR;
+                    const unsigned kd = to + key_at(t, chunk + 32 * u), vd = to + SIDE + value_at(t, chunk + 32 * u);
+                    const char* from_k = k[i / PER] + i % PER * 512;
+                    const char* from_v = v[i / PER] + i % PER * 512;
+                    if constexpr (decltype(whole)::value) {
+                        copy16(kd, from_k);
+                        copy16(vd, from_v);
+                    } else {
+                        copy16_or_zero(kd, from_k, seen >> t & 1u);
+                        copy16_or_zero(vd, from_v, seen >> t & 1u);
+                    }
+                }
+            };
+            if (seen == 0xffffffffu >> (32 - TOKENS)) copy(std::true_type());
+            else copy(std::false_type());
         } else {
             const int page = good >> lane & 1u ? (int)entry[0] : 0;
 #pragma unroll
@@ -260,9 +277,8 @@ struct Ring {
             int64_t at = 0;
             const bool mine = lane < TOKENS && (seen >> (lane % TOKENS) & 1u);
             if constexpr (PACKED) {
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-                    if (lane / BLOCK == b) at = entry[b] * p.ss[0] + (int64_t)(slot[b] + lane % BLOCK) * p.ss[2];
+                const bool second = NB > 1 && lane >= BLOCK;
+                at = (second ? entry[NB - 1] : entry[0]) * p.ss[0] + (int64_t)((second ? slot[NB - 1] : slot[0]) + lane % BLOCK) * p.ss[2];
             } else {
                 at = entry[0] * p.ss[0] + (int64_t)slot[0] * p.ss[2];
             }
@@ -282,9 +298,14 @@ struct Ring {
 // Lane (g, r) = (lane / 4, lane % 4).  Scores S = Q K^T: the lane's operand of K is 16 bytes of tokens g and 8 + g of 16; it
 // receives the scores of head g with tokens 2r, 2r + 1, 8 + 2r, 9 + 2r.  Values O = P V: weights of just these tokens are its
 // operand of P, and its operand of V is 16 (or 8) bytes of the same four tokens, two tokens' values interleaved by byte permutes.
-template <int DTYPE, int DP, bool PACKED>
+//
+// A tile of 8 heads has its upper terms in rows g and the next ones in rows g + 8, and bf16's lowest terms take a product of
+// their own.  A bf16 tile of 4 heads fits all three in one product: rows h, 4 + h and 8 + h.
+template <int DTYPE, int DP, int HT, bool PACKED>
 struct TensorWarp {
-    static constexpr int HEADS = 8;
+    static constexpr int HEADS = HT;
+    static constexpr bool THREE = HT == 4;       // three terms in one product
+    static_assert(HT == 8 || (HT == 4 && DTYPE == TE_KV_BF16), "tiles of 8 heads, or of 4 in bf16");
     static constexpr bool E4M3 = DTYPE == TE_KV_E4M3;
     static constexpr int ES = E4M3 ? 1 : 2;
     static constexpr int TOKENS = DP * ES <= 128 ? 32 : 16;             // 8 KB a stage (16 for bf16 rows of 256)
@@ -294,7 +315,7 @@ struct TensorWarp {
     static constexpr int VW = E4M3 && DP < 128 ? 8 : 16;                // bytes of a value a lane holds per chunk
     static constexpr int VE = VW / ES;                                  // elements of it
     static constexpr int VC = DP / (8 * VE);                            // chunks of 8 lanes
-    static constexpr int KQ = 4;                                        // left operands of Q per group, 16 bytes a lane each
+    static constexpr int KQ = THREE ? 2 : 4;                            // left operands of Q per group, 16 bytes a lane each
     static constexpr int Q_BYTES = KG * KQ * 32 * 16;
     static constexpr int MIN_BLOCKS = R::BYTES * WARPS > 110000 ? 1 : 2;
     static constexpr float LIFT = 10.0f;        // e4m3: weights reach 2^10, so that the lower of their two half terms keeps 2^-34 of the largest
@@ -319,16 +340,17 @@ struct TensorWarp {
         }
         // one thread per (group, lane, pair of elements); a left operand is {row g, row g + 8, row g, row g + 8} of pairs 2j, 2j, 2j + 1,
         // 2j + 1.  e4m3: operand j of 4 holds upper and lower terms.  bf16: operand j of 2 upper and middle ones, operand 2 + j lower ones
-        // (and zeros in row g + 8).
+        // (and zeros in row g + 8); a tile of 4 heads has upper terms in rows h, middle ones in 4 + h, lower ones in 8 + h.
         constexpr int PAIRS = E4M3 ? 8 : 4;
         for (int i = threadIdx.x; i < KG * 32 * PAIRS; i += THREADS) {
             const int j = i % PAIRS, lane = i / PAIRS % 32, c = i / PAIRS / 32;
             const int g = lane / 4, r = lane % 4;
             const int at = (E4M3 ? 64 * c + 16 * r : 32 * c + 8 * r) + 2 * j;
+            const int h = THREE ? g % 4 : g;
             float x = 0.0f, y = 0.0f;
-            if (g < s.heads && at < p.d) {
-                x = q[g * p.qs[1] + at];
-                y = q[g * p.qs[1] + at + 1];
+            if (h < s.heads && at < p.d) {
+                x = q[h * p.qs[1] + at];
+                y = q[h * p.qs[1] + at + 1];
             }
             unsigned* w = words + ((c * KQ + j / 2) * 32 + lane) * 4 + j % 2 * 2;
             if constexpr (E4M3) {
@@ -343,8 +365,14 @@ struct TensorWarp {
                 x -= bf16_lo(w[0]);
                 y -= bf16_hi(w[0]);
                 w[1] = pack_bf16(x, y);
-                w[2 * 32 * 4] = pack_bf16(x - bf16_lo(w[1]), y - bf16_hi(w[1]));
-                w[2 * 32 * 4 + 1] = 0u;
+                const unsigned low = pack_bf16(x - bf16_lo(w[1]), y - bf16_hi(w[1]));
+                if constexpr (THREE) {
+                    if (g >= 4) w[0] = w[1];
+                    w[1] = g < 4 ? low : 0u;
+                } else {
+                    w[2 * 32 * 4] = low;
+                    w[2 * 32 * 4 + 1] = 0u;
+                }
             }
         }
     }
@@ -400,28 +428,31 @@ struct TensorWarp {
             const char* values = keys + R::SIDE;
             const float* scales = reinterpret_cast<const float*>(keys + 2 * R::SIDE);
             // ---- scores
-            float sc[NK][2][4];
+            // (two chains of products for every 8 tokens: a product waits for the one before it in its chain)
+            float sc[2 * NK][2][4];
 #pragma unroll
             for (int c = 0; c < KG; ++c) {
                 const uint4* q = reinterpret_cast<const uint4*>(words) + c * KQ * 32 + lane;
-                const uint4 q0 = q[0], q1 = q[32], q2 = q[64], q3 = q[96];
+                uint4 qw[KQ];
+#pragma unroll
+                for (int i = 0; i < KQ; ++i) qw[i] = q[32 * i];
 #pragma unroll
                 for (int i = 0; i < 2 * NK; ++i) {
                     const uint4 x = *reinterpret_cast<const uint4*>(keys + R::key_at(i * 8 + g, 4 * c + r));
-                    float (&y)[4] = sc[i / 2][i % 2];
+                    float (&y)[4] = sc[i][0], (&z)[4] = sc[i][1];
                     if constexpr (E4M3) {
                         const uint2 k0 = halves_of_e4m3(x.x), k1 = halves_of_e4m3(x.y), k2 = halves_of_e4m3(x.z), k3 = halves_of_e4m3(x.w);
-                        if (c == 0) mma_from_zero<true>(y, q0, k0.x, k0.y);
-                        else mma<true>(y, q0, k0.x, k0.y);
-                        mma<true>(y, q1, k1.x, k1.y);
-                        mma<true>(y, q2, k2.x, k2.y);
-                        mma<true>(y, q3, k3.x, k3.y);
+                        mma_first_or_next<true>(c == 0, y, qw[0], k0.x, k0.y);
+                        mma_first_or_next<true>(c == 0, z, qw[1], k1.x, k1.y);
+                        mma<true>(y, qw[2], k2.x, k2.y);
+                        mma<true>(z, qw[3], k3.x, k3.y);
                     } else {
-                        if (c == 0) mma_from_zero<false>(y, q0, x.x, x.y);
-                        else mma<false>(y, q0, x.x, x.y);
-                        mma<false>(y, q2, x.x, x.y);
-                        mma<false>(y, q1, x.z, x.w);
-                        mma<false>(y, q3, x.z, x.w);
+                        mma_first_or_next<false>(c == 0, y, qw[0], x.x, x.y);
+                        mma_first_or_next<false>(c == 0, z, qw[1], x.z, x.w);
+                        if constexpr (!THREE) {
+                            mma<false>(y, qw[2], x.x, x.y);
+                            mma<false>(z, qw[3], x.z, x.w);
+                        }
                     }
                 }
             }
@@ -432,7 +463,10 @@ struct TensorWarp {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int t = nk * 16 + 8 * (i / 2) + 2 * r + i % 2;
-                    float x = (sc[nk][i / 2][i % 2] + sc[nk][i / 2][2 + i % 2]) * unit;
+                    const float (&y)[4] = sc[2 * nk + i / 2][0], (&z)[4] = sc[2 * nk + i / 2][1];
+                    float x = (y[i % 2] + z[i % 2]) + (y[2 + i % 2] + z[2 + i % 2]);
+                    if constexpr (THREE) x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    x *= unit;
                     if constexpr (E4M3) x *= scales[t];
                     w[nk][i] = seen[0] >> t & 1u ? x : -INFINITY;
                     top = fmaxf(top, w[nk][i]);
@@ -446,12 +480,12 @@ struct TensorWarp {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             top = fmaxf(top, m);
             const float base = settled(top);
-            float keep = exp2f(m - base), sum = 0.0f;
+            float keep = exp2_of(m - base), sum = 0.0f;
 #pragma unroll
             for (int nk = 0; nk < NK; ++nk)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = exp2f(w[nk][i] - base);
+                    const float e = exp2_of(w[nk][i] - base);
                     sum += e;
                     if constexpr (!E4M3) w[nk][i] = e;
                 }
@@ -462,11 +496,11 @@ struct TensorWarp {
                 topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 2));
                 topv = fmaxf(topv, mv);
                 const float basev = settled(topv);
-                keep = exp2f(mv - basev);
+                keep = exp2_of(mv - basev);
 #pragma unroll
                 for (int nk = 0; nk < NK; ++nk)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[nk][i] = exp2f(vs[nk][i] - basev + LIFT);
+                    for (int i = 0; i < 4; ++i) w[nk][i] = exp2_of(vs[nk][i] - basev + LIFT);
                 mv = topv;
             }
             uint4 a[NK], lower[NK];         // left operands of P; bf16: the lowest terms apart
@@ -486,6 +520,9 @@ struct TensorWarp {
                     a[nk].y = pack_bf16(x0, x1);
                     a[nk].w = pack_bf16(x2, x3);
                     lower[nk] = make_uint4(pack_bf16(x0 - bf16_lo(a[nk].y), x1 - bf16_hi(a[nk].y)), 0u, pack_bf16(x2 - bf16_lo(a[nk].w), x3 - bf16_hi(a[nk].w)), 0u);
+                    if constexpr (THREE) {      // heads' lanes hold upper and lower terms, the other half middle ones
+                        a[nk] = g < 4 ? make_uint4(a[nk].x, lower[nk].x, a[nk].z, lower[nk].z) : make_uint4(a[nk].y, 0u, a[nk].w, 0u);
+                    }
                 }
             }
             // ---- values
@@ -523,7 +560,7 @@ struct TensorWarp {
                                 const unsigned b0 = __byte_perm(x[nk][0][i], x[nk][1][i], e ? 0x7632 : 0x5410), b1 = __byte_perm(x[nk][2][i], x[nk][3][i], e ? 0x7632 : 0x5410);
                                 if (nk == 0) mma_from_zero<false>(y0, a[nk], b0, b1);
                                 else mma<false>(y0, a[nk], b0, b1);
-                                mma<false>(y0, lower[nk], b0, b1);
+                                if constexpr (!THREE) mma<false>(y0, lower[nk], b0, b1);
                             }
                         }
                         if constexpr (E4M3) {
@@ -544,17 +581,22 @@ struct TensorWarp {
         // one sum per head, and e4m3 sums measured against m like the others
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-        const float back = E4M3 ? exp2f(settled(mv) - settled(m) - LIFT) : 1.0f;
+        const float back = E4M3 ? exp2_of(settled(mv) - settled(m) - LIFT) : 1.0f;
 #pragma unroll
         for (int i = 0; i < VC * VE; ++i) {
             acc[i][0] *= back;
             acc[i][1] *= back;
+            if constexpr (THREE) {
+                acc[i][0] += __shfl_xor_sync(0xffffffffu, acc[i][0], 16);
+                acc[i][1] += __shfl_xor_sync(0xffffffffu, acc[i][1], 16);
+            }
         }
     }
 
     // This warp's sums into shared memory: acc [HEADS][DP], ml [HEADS].
     __device__ void put(float* out, float2* ml) const {
         const int lane = threadIdx.x % 32, g = lane / 4, r = lane % 4;
+        if (g >= HEADS) return;
         if (r == 0) ml[g] = make_float2(m, l);
 #pragma unroll
         for (int c = 0; c < VC; ++c)
@@ -682,13 +724,13 @@ struct FmaWarp {
                 }
 #pragma unroll
                 for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const float base = settled(top), keep = exp2f(m[j] - base);
+                const float base = settled(top), keep = exp2_of(m[j] - base);
                 l[j] *= keep;
                 moved |= top != m[j];
                 m[j] = top;
 #pragma unroll
                 for (int i = 0; i < TG; ++i) {
-                    const float e = exp2f(w[i] - base);
+                    const float e = exp2_of(w[i] - base);
                     l[j] += e;
                     weights[(g + 8 * i) * HT + h] = pair(e, e);
                 }
@@ -767,7 +809,7 @@ struct FmaWarp {
     }
 };
 
-template <int DTYPE, int DP, int HT, bool PACKED> struct WarpOf { typedef TensorWarp<DTYPE, DP, PACKED> type; };
+template <int DTYPE, int DP, int HT, bool PACKED> struct WarpOf { typedef TensorWarp<DTYPE, DP, HT, PACKED> type; };
 template <int DP, int HT, bool PACKED> struct WarpOf<TE_KV_F32, DP, HT, PACKED> { typedef FmaWarp<DP, HT, PACKED> type; };
 
 // ---------------------------------------------------------------------------------------------------- the two kernels
@@ -899,7 +941,7 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int j = 0; j < WARPS; ++j) {
-                const float f = exp2f(ml[j][h].x - base);
+                const float f = exp2_of(ml[j][h].x - base);
                 const float4 x = *reinterpret_cast<const float4*>(sums(j, h, c));
                 l += f * ml[j][h].y;
                 a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
@@ -949,7 +991,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(const AttnP
     for (int i = warp; i < count; i += JOIN_WARPS) {
         const int64_t o = at(i);
         const float2 ml = p.part_ml[o];
-        const float f = exp2f(ml.x - base);
+        const float f = exp2_of(ml.x - base);
         l += f * ml.y;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -979,9 +1021,12 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(const AttnP
 }
 
 // ------------------------------------------------------------------------------------------------------------ host side
-// Heads a tile holds: 8 on the tensor cores; with FMAs the smallest of 1, 2, 4, 8 that takes the group, since every head
-// of a tile is computed whether it is there or not.
-int heads_per_tile(int dtype, int64_t group) { return dtype != TE_KV_F32 ? 8 : group >= 5 ? 8 : group >= 3 ? 4 : (int)group; }
+// Heads a tile holds.  Every head of a tile is computed whether it is there or not, so: with FMAs the smallest of 1, 2, 4, 8
+// that takes the group; on the tensor cores 4 where that takes it in bf16 (half the products), else 8.
+int heads_per_tile(int dtype, int64_t group) {
+    if (dtype == TE_KV_E4M3 || group >= 5) return 8;
+    return dtype == TE_KV_BF16 || group >= 3 ? 4 : (int)group;
+}
 
 // Thread blocks per SM: two where two rings fit the shared memory, one for the longest rows.
 int blocks_per_sm(int dtype, int64_t d) { return dtype == TE_KV_E4M3 || d <= 128 ? 2 : 1; }
@@ -1015,6 +1060,7 @@ cudaError_t launch_tiles(te_b200_ctx* ctx, const AttnParams& p, int workers, cud
 
 template <int DP>
 cudaError_t launch_width(te_b200_ctx* ctx, const AttnParams& p, int dtype, int heads, int workers, cudaStream_t st) {
+    if (dtype == TE_KV_BF16 && heads == 4) return launch_tiles<TE_KV_BF16, DP, 4>(ctx, p, workers, st);
     if (dtype == TE_KV_BF16) return launch_tiles<TE_KV_BF16, DP, 8>(ctx, p, workers, st);
     if (dtype == TE_KV_E4M3) return launch_tiles<TE_KV_E4M3, DP, 8>(ctx, p, workers, st);
     if (heads == 1) return launch_tiles<TE_KV_F32, DP, 1>(ctx, p, workers, st);
