@@ -231,13 +231,14 @@ def test_eight_bit_grid_of_the_reference():
 
 
 def test_shares_of_paged_attention_on_the_host(tmp_path):
-    """Every tile of every segment belongs to exactly one worker, a segment's workers are those that the join adds up, and
-    no worker holds more than one part of either kind."""
+    """Going through all workers' pieces covers every tile of every segment once and in order, the parts of a segment lie in
+    the places that the join adds up, and no place is used twice."""
     src = tmp_path / "shares.cpp"
     src.write_text(r"""
 #include <stdio.h>
 #include <algorithm>
 #include <map>
+#include <utility>
 #include <vector>
 #include "paged_plan.h"
 using namespace te;
@@ -245,34 +246,68 @@ int main() {
     long bad = 0;
     uint64_t x = 88172645463325252ull;
     auto rnd = [&](uint64_t n) { x ^= x << 13; x ^= x >> 7; x ^= x << 17; return x % n; };
-    for (int trial = 0; trial < 3000; ++trial) {
+    for (int trial = 0; trial < 4000; ++trial) {
         const int tile = trial % 2 ? 64 : 32, heads = 1 + (int)rnd(9), rows = 1 + (int)rnd(12), grid = 1 + (int)rnd(trial % 3 ? 300 : 7);
         const int64_t window = rnd(3) ? 0 : 1 + (int64_t)rnd(500), most = 3000;
-        int64_t units = 0;
-        std::vector<int64_t> begin, end;            // of segments with tiles
+        std::vector<int64_t> len(rows), row_begin(rows + 1, 0);
         for (int r = 0; r < rows; ++r) {
-            const int64_t len = (int64_t)rnd(8) == 0 ? -(int64_t)rnd(3) : (int64_t)rnd(trial % 5 ? 3500 : 70);
-            const RowRange range = row_range(len, most, window);
-            bad += range.n != std::max<int64_t>(0, std::min(len, most)) || range.first != (window ? std::max<int64_t>(0, range.n - window) : 0);
+            len[r] = (int64_t)rnd(8) == 0 ? -(int64_t)rnd(3) : (int64_t)rnd(trial % 5 ? 3500 : 70);
+            const RowRange range = row_range(len[r], most, window);
+            bad += range.n != std::max<int64_t>(0, std::min(len[r], most)) || range.first != (window ? std::max<int64_t>(0, range.n - window) : 0);
             const int c = row_tiles(range, tile);
             if (range.n > range.first) bad += c != (range.n - 1) / tile - range.first / tile + 1; else bad += c != 0;
-            for (int h = 0; h < heads && c; ++h) { begin.push_back(units); units += c; end.push_back(units); }
+            row_begin[r + 1] = row_begin[r] + (int64_t)segment_units(c) * heads;
         }
+        const int64_t units = row_begin[rows];
         if (!units) continue;
+        auto range_of = [&](int r) { return row_range(len[r], most, window); };
         const int workers = (int)std::min<int64_t>(grid, units);
         bad += worker_begin(units, workers, 0) != 0 || worker_begin(units, workers, workers) != units;
-        for (int w = 0; w < workers; ++w) bad += worker_begin(units, workers, w + 1) <= worker_begin(units, workers, w);
-        for (int64_t u = 0; u < units; ++u) {
-            const int w = worker_of(units, workers, u);
-            bad += w < 0 || w >= workers || u < worker_begin(units, workers, w) || u >= worker_begin(units, workers, w + 1);
+        std::map<std::pair<int, int>, int64_t> done;                        // (row, head tile) -> tiles covered so far
+        std::map<int, std::pair<int, int>> place;                           // part slot -> its segment
+        std::map<std::pair<int, int>, std::vector<int>> parts;              // segment -> slots in order of its tiles
+        std::map<std::pair<int, int>, std::pair<int, int>> join;            // segment -> first and last worker
+        for (int w = 0; w < workers; ++w) {
+            const int64_t u0 = worker_begin(units, workers, w), u1 = worker_begin(units, workers, w + 1);
+            bad += u1 <= u0 || worker_of(units, workers, u0) != w || worker_of(units, workers, u1 - 1) != w;
+            int r = 0;
+            while (row_begin[r + 1] <= u0) ++r;
+            Walker walk;
+            walk.start(u0, u1, r, row_begin[r]);
+            Piece p;
+            int last_row = -1, last_head = -1;
+            while (walk.next(range_of, heads, tile, p)) {
+                const std::pair<int, int> seg(p.row, p.head_tile);
+                const RowRange range = range_of(p.row);
+                const int tiles = row_tiles(range, tile);
+                bad += p.row < 0 || p.row >= rows || p.head_tile < 0 || p.head_tile >= heads || p.tiles < 1 || p.range.n != range.n || p.range.first != range.first;
+                bad += p.first_tile != range.first / tile + done[seg];          // in order, without gaps
+                bad += p.begins != (done[seg] == 0);
+                done[seg] += p.tiles;
+                bad += p.ends != (done[seg] == tiles) || done[seg] > tiles;
+                bad += p.segment_end != row_begin[p.row] + (int64_t)(p.head_tile + 1) * segment_units(tiles);
+                bad += p.row < last_row || (p.row == last_row && p.head_tile <= last_head);
+                last_row = p.row; last_head = p.head_tile;
+                if (!(p.begins && p.ends)) {
+                    const int slot = part_slot(w, p.begins);
+                    bad += place.count(slot) || slot < 0 || slot >= 2 * workers;
+                    place[slot] = seg;
+                    parts[seg].push_back(slot);
+                }
+                if (p.begins && !p.ends) join[seg] = std::make_pair(w, worker_of(units, workers, p.segment_end - 1));
+            }
         }
-        std::map<int, int> used;
-        for (size_t s = 0; s < begin.size(); ++s) {
-            const int first = worker_of(units, workers, begin[s]), last = worker_of(units, workers, end[s] - 1);
-            if (first == last) continue;
-            for (int w = first; w <= last; ++w) used[part_slot(w, w == first)]++;
-        }
-        for (auto& u : used) bad += u.second != 1 || u.first < 0 || u.first >= 2 * workers;
+        for (int r = 0; r < rows; ++r)
+            for (int h = 0; h < heads; ++h) {
+                const int tiles = row_tiles(range_of(r), tile);
+                const std::pair<int, int> seg(r, h);
+                bad += done[seg] != tiles;
+                if (!parts.count(seg)) { bad += join.count(seg); continue; }
+                const std::pair<int, int> j = join.at(seg);
+                std::vector<int> want;
+                for (int w = j.first; w <= j.second; ++w) want.push_back(part_slot(w, w == j.first));
+                bad += want != parts[seg];
+            }
     }
     printf("%ld\n", bad);
     return 0;

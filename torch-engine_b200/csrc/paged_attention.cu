@@ -61,10 +61,18 @@ struct AttnParams {
     int* status;
 };
 
-struct Segment {
-    int row, kv_head, head0, heads;       // query heads head0 .. head0 + heads - 1
-    RowRange range;
+struct Heads {
+    int kv_head, head0, count;       // query heads head0 .. head0 + count - 1
 };
+template <int HT>
+__device__ __forceinline__ Heads heads_of(const AttnParams& p, int head_tile) {
+    Heads h;
+    h.kv_head = head_tile / p.head_tiles;
+    const int part = head_tile % p.head_tiles * HT;
+    h.head0 = h.kv_head * p.group + part;
+    h.count = min(HT, p.group - part);
+    return h;
+}
 
 // ---------------------------------------------------------------------------------------------------- small pieces
 // c += a b, and c = a b; a holds the four words of the left operand.
@@ -186,17 +194,15 @@ struct Ring {
     int64_t entry[NB];          // of the page table, as read, for the stage to be issued next
     unsigned slot[NB];
 
-    __device__ __forceinline__ const char* stage(const char* ring, int i) const { return ring + i * STAGE; }
-
     // Reads the page table for the tokens from t0 on; lane's own token (!PACKED), or the page of each block.
-    __device__ __forceinline__ void look_up(const AttnParams& p, const int64_t* table, int64_t t0, int64_t t_end, int64_t n) {
+    __device__ __forceinline__ void look_up(const AttnParams& p, const int64_t* table, int64_t t0, int64_t n) {
         const int lane = threadIdx.x % 32;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const int64_t t = t0 + (PACKED ? b * BLOCK : lane % TOKENS);
             entry[b] = -1;
             slot[b] = 0;
-            if (t0 < t_end && t < n) {                 // n is within the table
+            if (t < n) {                               // n is within the table
                 const unsigned i = fast_quotient((unsigned)t, p.page_size);
                 slot[b] = (unsigned)t - i * p.page_size.divisor;
                 entry[b] = __ldg(table + i);
@@ -320,58 +326,74 @@ struct TensorWarp {
     static constexpr int MIN_BLOCKS = R::BYTES * WARPS > 110000 ? 1 : 2;
     static constexpr float LIFT = 10.0f;        // e4m3: weights reach 2^10, so that the lower of their two half terms keeps 2^-34 of the largest
 
-    // Splits the tile's queries into terms, in the order the tensor operand wants them.  q_unit: e4m3 only, what the scores of a head
-    // are measured in (the terms are the query brought to below 2^13 by a power of two).
-    static __device__ void stage_queries(const AttnParams& p, const Segment& s, unsigned* words, float* q_unit) {
-        const float* q = p.q + s.row * p.qs[0] + s.head0 * p.qs[1];
-        if constexpr (E4M3) {
-            const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-            for (int h = warp; h < HEADS; h += WARPS) {
+    static constexpr int QH = HEADS / WARPS, QP = DP / 64;               // heads a warp splits, pairs of elements a lane
+
+    // Queries into registers ahead of split_queries: heads warp, warp + 4 of the tile, lane's pairs of elements.
+    struct Queries {
+        float x[QH][QP][2];
+    };
+    static __device__ __forceinline__ void load_queries(Queries& w, const AttnParams& p, int row, const Heads& heads) {
+        const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+#pragma unroll
+        for (int i = 0; i < QH; ++i) {
+            const int h = warp + WARPS * i;
+            const float* q = p.q + row * p.qs[0] + (heads.head0 + h) * p.qs[1];
+#pragma unroll
+            for (int k = 0; k < QP; ++k) {
+                const int c = 2 * (lane + 32 * k);
+                const bool there = h < heads.count && c < p.d;
+                w.x[i][k][0] = there ? q[c] : 0.0f;
+                w.x[i][k][1] = there ? q[c + 1] : 0.0f;
+            }
+        }
+    }
+    // Splits them into terms, in the order the left operand wants: {row g, row g + 8, row g, row g + 8} of pairs 2j, 2j, 2j + 1, 2j + 1
+    // of a lane's 16 bytes.  e4m3: operand j of 4 holds upper and lower terms of the query, brought to below 2^13 by a power of two that
+    // q_unit keeps.  bf16: operand j of 2 holds upper and middle terms, operand 2 + j lower ones (and zeros in row g + 8); a tile of 4
+    // heads has upper terms in rows h, middle ones in 4 + h, lower ones in 8 + h.
+    static __device__ __forceinline__ void split_queries(const Queries& w, unsigned* words, float* q_unit) {
+        const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+#pragma unroll
+        for (int i = 0; i < QH; ++i) {
+            const int h = warp + WARPS * i;
+            float unit = 1.0f;
+            if constexpr (E4M3) {
                 float top = 0.0f;
-                if (h < s.heads)
-                    for (int c = lane; c < p.d; c += 32) top = fmaxf(top, fabsf(q[h * p.qs[1] + c]));
+#pragma unroll
+                for (int k = 0; k < QP; ++k) top = fmaxf(top, fmaxf(fabsf(w.x[i][k][0]), fabsf(w.x[i][k][1])));
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 int e = (int)(__float_as_uint(top) >> 23) - 126 - 13;          // top < 2^(e + 13)
-                e = e < -100 ? -100 : e > 100 ? 100 : e;
-                if (lane == 0) q_unit[h] = __uint_as_float((unsigned)(e + 127) << 23);
+                e = e < -100 ? -100 : e;
+                unit = __uint_as_float((unsigned)(127 - e) << 23);
+                if (lane == 0) q_unit[h] = __uint_as_float((unsigned)(127 + e) << 23);
             }
-            __syncthreads();
-        }
-        // one thread per (group, lane, pair of elements); a left operand is {row g, row g + 8, row g, row g + 8} of pairs 2j, 2j, 2j + 1,
-        // 2j + 1.  e4m3: operand j of 4 holds upper and lower terms.  bf16: operand j of 2 upper and middle ones, operand 2 + j lower ones
-        // (and zeros in row g + 8); a tile of 4 heads has upper terms in rows h, middle ones in 4 + h, lower ones in 8 + h.
-        constexpr int PAIRS = E4M3 ? 8 : 4;
-        for (int i = threadIdx.x; i < KG * 32 * PAIRS; i += THREADS) {
-            const int j = i % PAIRS, lane = i / PAIRS % 32, c = i / PAIRS / 32;
-            const int g = lane / 4, r = lane % 4;
-            const int at = (E4M3 ? 64 * c + 16 * r : 32 * c + 8 * r) + 2 * j;
-            const int h = THREE ? g % 4 : g;
-            float x = 0.0f, y = 0.0f;
-            if (h < s.heads && at < p.d) {
-                x = q[h * p.qs[1] + at];
-                y = q[h * p.qs[1] + at + 1];
-            }
-            unsigned* w = words + ((c * KQ + j / 2) * 32 + lane) * 4 + j % 2 * 2;
-            if constexpr (E4M3) {
-                const float unit = 1.0f / q_unit[g];                   // a power of two
-                x *= unit;
-                y *= unit;
-                w[0] = pack_half(x, y);
-                const float2 f = unpack_half(w[0]);
-                w[1] = pack_half(x - f.x, y - f.y);
-            } else {
-                w[0] = pack_bf16(x, y);
-                x -= bf16_lo(w[0]);
-                y -= bf16_hi(w[0]);
-                w[1] = pack_bf16(x, y);
-                const unsigned low = pack_bf16(x - bf16_lo(w[1]), y - bf16_hi(w[1]));
-                if constexpr (THREE) {
-                    if (g >= 4) w[0] = w[1];
-                    w[1] = g < 4 ? low : 0u;
+#pragma unroll
+            for (int k = 0; k < QP; ++k) {
+                constexpr int GROUP = E4M3 ? 64 : 32, LANE = GROUP / 4;
+                const int at = 2 * (lane + 32 * k), c = at / GROUP, r = at % GROUP / LANE, j = at % LANE / 2;
+                unsigned* out = words + ((c * KQ + j / 2) * 32 + 4 * h + r) * 4 + j % 2 * 2;
+                float x = w.x[i][k][0] * unit, y = w.x[i][k][1] * unit;
+                if constexpr (E4M3) {
+                    const unsigned upper = pack_half(x, y);
+                    const float2 f = unpack_half(upper);
+                    out[0] = upper;
+                    out[1] = pack_half(x - f.x, y - f.y);
                 } else {
-                    w[2 * 32 * 4] = low;
-                    w[2 * 32 * 4 + 1] = 0u;
+                    const unsigned upper = pack_bf16(x, y);
+                    x -= bf16_lo(upper);
+                    y -= bf16_hi(upper);
+                    const unsigned middle = pack_bf16(x, y), lower = pack_bf16(x - bf16_lo(middle), y - bf16_hi(middle));
+                    out[0] = upper;
+                    if constexpr (THREE) {
+                        out[1] = lower;
+                        out[4 * 4 * 4] = middle;        // four rows on: 4 x 4 lanes
+                        out[4 * 4 * 4 + 1] = 0u;
+                    } else {
+                        out[1] = middle;
+                        out[2 * 32 * 4] = lower;
+                        out[2 * 32 * 4 + 1] = 0u;
+                    }
                 }
             }
         }
@@ -380,6 +402,7 @@ struct TensorWarp {
     float acc[VC * VE][2];     // [n tile][2 columns] of head g, both rows of its terms
     float m, l;                // of head g; l over this lane's tokens only
     float mv;                  // e4m3: the maximum the values' weights are measured against
+    float unit;                // what a score is multiplied by
 
     // The tensor core truncates as it adds to its accumulator, which over many tokens would shrink the sums; so each 16 tokens'
     // product starts from zero and is added here, rounded to nearest, with the rescaling in the same FMA.
@@ -388,45 +411,20 @@ struct TensorWarp {
         acc[i][1] = fmaf(acc[i][1], keep, x[1] + x[3]);
     }
 
-    __device__ void run(const AttnParams& p, const Segment& s, const unsigned* words, const float* q_unit, char* ring, int64_t tile, int64_t tile_end) {
-        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, r = lane % 4;
-        const int64_t* table = p.page_table + s.row * p.table_stride;
-        const RowRange range = s.range;
-        int64_t t0 = tile * R::STEP + warp * TOKENS;               // of the stage to be issued
-        const int64_t t_end = tile_end * R::STEP;
-        const int stages = (int)((tile_end - tile));               // every warp has one stage of each tile
+    __device__ __forceinline__ void begin(const AttnParams& p, const float* q_unit) {
 #pragma unroll
         for (int i = 0; i < VC * VE; ++i) acc[i][0] = acc[i][1] = 0.0f;
         m = mv = -INFINITY;
         l = 0.0f;
-        const float unit = p.scale * LOG2E * (E4M3 ? q_unit[g] : 1.0f);
-        R copies;
-        copies.base = smem_address(ring);
-        unsigned seen[R::STAGES];
-        copies.look_up(p, table, t0, t_end, range.n);
-#pragma unroll
-        for (int i = 0; i < R::STAGES - 1; ++i) {
-            seen[i] = 0u;
-            if (i < stages) {
-                seen[i] = copies.issue(p, range, s.kv_head, t0, i);
-                t0 += R::STEP;
-                copies.look_up(p, table, t0, t_end, range.n);
-            }
-            copies_issued();
-        }
-        int at = 0, to = R::STAGES - 1;
-        for (int n = 0; n < stages; ++n) {
-            copies_wait<R::STAGES - 2>();
-            __syncwarp();                  // this stage has landed for all lanes, and all are done with the one before it
-            if (t0 < t_end) {
-                seen[R::STAGES - 1] = copies.issue(p, range, s.kv_head, t0, to);
-                t0 += R::STEP;
-                copies.look_up(p, table, t0, t_end, range.n);
-            }
-            copies_issued();
-            const char* keys = copies.stage(ring, at);
-            const char* values = keys + R::SIDE;
-            const float* scales = reinterpret_cast<const float*>(keys + 2 * R::SIDE);
+        unit = p.scale * LOG2E * (E4M3 ? q_unit[threadIdx.x % 32 / 4] : 1.0f);
+    }
+
+    // One stage's tokens, those of the bits of `seen`.
+    __device__ __forceinline__ void step(const char* keys, unsigned seen, const unsigned* words) {
+        const int lane = threadIdx.x % 32, g = lane / 4, r = lane % 4;
+        const char* values = keys + R::SIDE;
+        const float* scales = reinterpret_cast<const float*>(keys + 2 * R::SIDE);
+        {
             // ---- scores
             // (two chains of products for every 8 tokens: a product waits for the one before it in its chain)
             float sc[2 * NK][2][4];
@@ -468,7 +466,7 @@ struct TensorWarp {
                     if constexpr (THREE) x += __shfl_xor_sync(0xffffffffu, x, 16);
                     x *= unit;
                     if constexpr (E4M3) x *= scales[t];
-                    w[nk][i] = seen[0] >> t & 1u ? x : -INFINITY;
+                    w[nk][i] = seen >> t & 1u ? x : -INFINITY;
                     top = fmaxf(top, w[nk][i]);
                     if constexpr (E4M3) {       // a value's scale goes into its weight: 2^e, e from the exponent field
                         vs[nk][i] = w[nk][i] + (float)((int)(__float_as_uint(scales[TOKENS + t]) >> 23) - 127);
@@ -571,13 +569,11 @@ struct TensorWarp {
                         }
                     }
             }
-#pragma unroll
-            for (int i = 0; i + 1 < R::STAGES; ++i) seen[i] = seen[i + 1];
-            at = at + 1 == R::STAGES ? 0 : at + 1;
-            to = to + 1 == R::STAGES ? 0 : to + 1;
         }
-        copies_wait<0>();
-        __syncwarp();                      // the ring is free for the sums
+    }
+
+    // What is left to do when the last stage has been seen.
+    __device__ __forceinline__ void finish() {
         // one sum per head, and e4m3 sums measured against m like the others
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -594,7 +590,7 @@ struct TensorWarp {
     }
 
     // This warp's sums into shared memory: acc [HEADS][DP], ml [HEADS].
-    __device__ void put(float* out, float2* ml) const {
+    __device__ __forceinline__ void put(float* out, float2* ml) const {
         const int lane = threadIdx.x % 32, g = lane / 4, r = lane % 4;
         if (g >= HEADS) return;
         if (r == 0) ml[g] = make_float2(m, l);
@@ -629,60 +625,50 @@ struct FmaWarp {
                                                                                      // doubled for two FMAs at once
     static constexpr int MIN_BLOCKS = R::BYTES * WARPS > 110000 ? 1 : 2;
 
-    static __device__ void stage_queries(const AttnParams& p, const Segment& s, float* words) {
-        const float* q = p.q + s.row * p.qs[0] + s.head0 * p.qs[1];
-        for (int i = threadIdx.x; i < HT * DP; i += THREADS) {
-            const int h = i / DP, c = i % DP;
-            words[i] = h < s.heads && c < p.d ? q[h * p.qs[1] + c] : 0.0f;
+    static constexpr int QN = (HT * DP + THREADS - 1) / THREADS;
+
+    struct Queries {
+        float x[QN];
+    };
+    static __device__ __forceinline__ void load_queries(Queries& w, const AttnParams& p, int row, const Heads& heads) {
+        const float* q = p.q + row * p.qs[0] + heads.head0 * p.qs[1];
+#pragma unroll
+        for (int k = 0; k < QN; ++k) {
+            const int i = threadIdx.x + k * THREADS, h = i / DP, c = i % DP;
+            w.x[k] = h < heads.count && c < p.d ? q[h * p.qs[1] + c] : 0.0f;
+        }
+    }
+    static __device__ __forceinline__ void split_queries(const Queries& w, unsigned* words, float*) {
+#pragma unroll
+        for (int k = 0; k < QN; ++k) {
+            const int i = threadIdx.x + k * THREADS;
+            if (i < HT * DP) reinterpret_cast<float*>(words)[i] = w.x[k];
         }
     }
 
     unsigned long long acc[HT][VC][2];
     float m[OWN], l[OWN];          // of heads r, r + 4 (modulo HT); l over this lane's tokens only
 
-    __device__ void run(const AttnParams& p, const Segment& s, const float* q, char* ring, int64_t tile, int64_t tile_end) {
-        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, r = lane % 4;
-        const int64_t* table = p.page_table + s.row * p.table_stride;
-        const RowRange range = s.range;
-        int64_t t0 = tile * R::STEP + warp * TOKENS;               // of the stage to be issued
-        const int64_t t_end = tile_end * R::STEP;
-        const int stages = (int)(tile_end - tile);                 // every warp has one stage of each tile
-        unsigned long long* weights = reinterpret_cast<unsigned long long*>(const_cast<float*>(q) + HT * DP) + warp * (TOKENS * HT + HT);
-        unsigned long long* factors = weights + TOKENS * HT;
+    float unit;                    // what a score is multiplied by
+
+    __device__ __forceinline__ void begin(const AttnParams& p, const float*) {
 #pragma unroll
         for (int h = 0; h < HT; ++h)
 #pragma unroll
             for (int c = 0; c < VC; ++c) acc[h][c][0] = acc[h][c][1] = 0ull;
 #pragma unroll
         for (int i = 0; i < OWN; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
+        unit = p.scale * LOG2E;
+    }
+
+    __device__ __forceinline__ void step(const char* keys, unsigned seen, unsigned* words) {
+        const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, r = lane % 4;
         const int along = lane % LPT, which = lane / LPT;
-        const float unit = p.scale * LOG2E;
-        R copies;
-        copies.base = smem_address(ring);
-        unsigned seen[R::STAGES];
-        copies.look_up(p, table, t0, t_end, range.n);
-#pragma unroll
-        for (int i = 0; i < R::STAGES - 1; ++i) {
-            seen[i] = 0u;
-            if (i < stages) {
-                seen[i] = copies.issue(p, range, s.kv_head, t0, i);
-                t0 += R::STEP;
-                copies.look_up(p, table, t0, t_end, range.n);
-            }
-            copies_issued();
-        }
-        int at = 0, to = R::STAGES - 1;
-        for (int n = 0; n < stages; ++n) {
-            copies_wait<R::STAGES - 2>();
-            __syncwarp();                  // this stage has landed for all lanes, and all are done with the one before it
-            if (t0 < t_end) {
-                seen[R::STAGES - 1] = copies.issue(p, range, s.kv_head, t0, to);
-                t0 += R::STEP;
-                copies.look_up(p, table, t0, t_end, range.n);
-            }
-            copies_issued();
-            const char* keys = copies.stage(ring, at);
-            const char* values = keys + R::SIDE;
+        const char* values = keys + R::SIDE;
+        const float* q = reinterpret_cast<const float*>(words);
+        unsigned long long* weights = reinterpret_cast<unsigned long long*>(words + HT * DP) + warp * (TOKENS * HT + HT);
+        unsigned long long* factors = weights + TOKENS * HT;
+        {
             // ---- scores: every lane of a quad ends with the sums of all heads
             float sc[TG][HT];
 #pragma unroll
@@ -719,7 +705,7 @@ struct FmaWarp {
                     float x = sc[i][(4 * j) % HT];
 #pragma unroll
                     for (int u = 1; u < 4; ++u) x = r == u ? sc[i][(u + 4 * j) % HT] : x;
-                    w[i] = seen[0] >> (g + 8 * i) & 1u ? x * unit : -INFINITY;
+                    w[i] = seen >> (g + 8 * i) & 1u ? x * unit : -INFINITY;
                     top = fmaxf(top, w[i]);
                 }
 #pragma unroll
@@ -765,13 +751,11 @@ struct FmaWarp {
                     }
                 }
             }
-#pragma unroll
-            for (int i = 0; i + 1 < R::STAGES; ++i) seen[i] = seen[i + 1];
-            at = at + 1 == R::STAGES ? 0 : at + 1;
-            to = to + 1 == R::STAGES ? 0 : to + 1;
+            __syncwarp();                  // the weights have been read
         }
-        copies_wait<0>();
-        __syncwarp();                      // the ring is free for the sums
+    }
+
+    __device__ __forceinline__ void finish() {
 #pragma unroll
         for (int j = 0; j < OWN; ++j)
 #pragma unroll
@@ -790,7 +774,7 @@ struct FmaWarp {
                     }
     }
 
-    __device__ void put(float* out, float2* ml) const {
+    __device__ __forceinline__ void put(float* out, float2* ml) const {
         const int lane = threadIdx.x % 32, g = lane / 4, r = lane % 4;
 #pragma unroll
         for (int j = 0; j < OWN; ++j)
@@ -819,10 +803,9 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     typedef typename Warp::R R;
     constexpr int HEADS = Warp::HEADS, TILE = R::STEP;
     extern __shared__ __align__(128) char shared[];
-    char* rings = shared;                                  // [WARPS][R::BYTES]; at a segment's end each warp's sums
-    char* query = shared + WARPS * R::BYTES;               // [Warp::Q_BYTES]
-    static_assert(HEADS * DP * 4 <= R::BYTES, "a warp's sums fit its ring");
-    auto sums = [&](int j, int h, int c) { return reinterpret_cast<float*>(rings + j * R::BYTES) + h * DP + c; };
+    char* rings = shared;                                  // [WARPS][R::BYTES]
+    unsigned* query = reinterpret_cast<unsigned*>(shared + WARPS * R::BYTES);       // [Warp::Q_BYTES]
+    static_assert(HEADS * DP * 4 <= R::STAGE, "a warp's sums fit the stage it read last");
     __shared__ float2 ml[WARPS][HEADS];
     __shared__ float q_unit[HEADS];
     __shared__ int64_t scan[WARPS];
@@ -834,7 +817,9 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     const int tiles_of_heads = p.kv_heads * p.head_tiles;
     const int64_t most = p.max_pages * (int64_t)p.page_size.divisor;
 
-    // ---- this worker's share: the rows' tile counts, added up by all threads over slabs of rows
+    auto range_of = [&](int r) { return row_range(p.lens[r], most, p.window); };
+
+    // ---- this worker's share: the rows' units, added up by all threads over slabs of rows
     const int slab = (p.rows + THREADS - 1) / THREADS;
     const int r0 = min(p.rows, tid * slab), r1 = min(p.rows, r0 + slab);
     int64_t mine = 0;
@@ -842,7 +827,7 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     for (int r = r0; r < r1; ++r) {
         const int64_t len = p.lens[r];
         cut |= len > most;
-        mine += row_tiles(row_range(len, most, p.window), TILE);
+        mine += segment_units(row_tiles(row_range(len, most, p.window), TILE));
     }
     if (cut) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
     int64_t before = mine;
@@ -863,13 +848,13 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     }
     const int64_t units = total * tiles_of_heads;
     const int workers = (int)(units < gridDim.x ? units : (int64_t)gridDim.x);      // every one of them has a unit
-    int64_t unit = w < workers ? worker_begin(units, workers, w) : 0;
+    const int64_t unit = w < workers ? worker_begin(units, workers, w) : 0;
     const int64_t unit_end = w < workers ? worker_begin(units, workers, w + 1) : 0;
     if (unit < unit_end) {
-        const int64_t at = unit / tiles_of_heads;          // in tiles of rows
+        const int64_t at = unit / tiles_of_heads;          // in the rows' sums
         if (at >= before && at < before + mine) {
             for (int r = r0; r < r1; ++r) {
-                const int c = row_tiles(row_range(p.lens[r], most, p.window), TILE);
+                const int c = segment_units(row_tiles(range_of(r), TILE));
                 if (at < before + c) {
                     found_row = r;
                     found_prefix = before;
@@ -883,55 +868,73 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     __syncthreads();
     // rows without tokens
     for (int r = w; r < p.rows; r += gridDim.x) {
-        if (row_tiles(row_range(p.lens[r], most, p.window), TILE) > 0) continue;
+        if (row_tiles(range_of(r), TILE) > 0) continue;
         for (int i = tid; i < p.q_heads * p.d; i += THREADS) p.o[r * p.os[0] + i / p.d * p.os[1] + i % p.d] = 0.0f;
         if (p.lse)
             for (int i = tid; i < p.q_heads; i += THREADS) p.lse[(int64_t)r * p.q_heads + i] = -INFINITY;
     }
     if (unit >= unit_end) return;
 
-    // ---- its segments
-    int row = found_row;
-    int64_t row_begin = found_prefix * tiles_of_heads;     // first unit of the row
-    while (unit < unit_end) {
-        Segment s;
-        s.row = row;
-        s.range = row_range(p.lens[row], most, p.window);
-        const int tiles = row_tiles(s.range, TILE);
-        if (tiles == 0) { ++row; continue; }
-        const int64_t in_row = unit - row_begin;
-        const int ht = (int)(in_row / tiles);
-        if (ht >= tiles_of_heads) {
-            row_begin += (int64_t)tiles * tiles_of_heads;
-            ++row;
-            continue;
+    // ---- its pieces of segments.  Copies run two stages ahead of the arithmetic, into the next pieces as well, so each side
+    // goes through the pieces by itself.
+    Walker behind;
+    behind.start(unit, unit_end, found_row, found_prefix * tiles_of_heads);
+    Walker ahead = behind;
+    Piece piece, soon;
+    if (!behind.next(range_of, tiles_of_heads, TILE, piece)) return;        // a share that lies in a segment's SEGMENT_COST
+    ahead.next(range_of, tiles_of_heads, TILE, soon);
+    char* ring = rings + warp * R::BYTES;
+    R copies;
+    copies.base = smem_address(ring);
+    int64_t t0 = soon.first_tile * TILE + warp * R::TOKENS;                  // of this warp's next stage
+    copies.look_up(p, p.page_table + soon.row * p.table_stride, t0, soon.range.n);
+    auto issue_next = [&](int stage) {
+        unsigned seen = 0u;
+        if (soon.tiles > 0) {
+            seen = copies.issue(p, soon.range, soon.head_tile / p.head_tiles, t0, stage);
+            t0 += TILE;
+            if (--soon.tiles == 0 && ahead.next(range_of, tiles_of_heads, TILE, soon)) t0 = soon.first_tile * TILE + warp * R::TOKENS;
+            if (soon.tiles > 0) copies.look_up(p, p.page_table + soon.row * p.table_stride, t0, soon.range.n);
         }
-        const int64_t seg_begin = row_begin + (int64_t)ht * tiles, seg_end = seg_begin + tiles;
-        const int64_t stop = unit_end < seg_end ? unit_end : seg_end;
-        s.kv_head = ht / p.head_tiles;
-        const int part = ht % p.head_tiles * HEADS;
-        s.head0 = s.kv_head * p.group + part;
-        s.heads = min(HEADS, p.group - part);
-        const int64_t tile0 = s.range.first / TILE + (unit - seg_begin), tile1 = s.range.first / TILE + (stop - seg_begin);
-        {
-            Warp mywarp;
-            char* ring = rings + warp * R::BYTES;
-            if constexpr (DTYPE == TE_KV_F32) {
-                Warp::stage_queries(p, s, reinterpret_cast<float*>(query));
-                __syncthreads();
-                mywarp.run(p, s, reinterpret_cast<const float*>(query), ring, tile0, tile1);
-            } else {
-                Warp::stage_queries(p, s, reinterpret_cast<unsigned*>(query), q_unit);
-                __syncthreads();
-                mywarp.run(p, s, reinterpret_cast<const unsigned*>(query), q_unit, ring, tile0, tile1);
-            }
-            mywarp.put(sums(warp, 0, 0), ml[warp]);
+        copies_issued();
+        return seen;
+    };
+    Heads heads = heads_of<HEADS>(p, piece.head_tile);
+    typename Warp::Queries loaded;
+    Warp::load_queries(loaded, p, piece.row, heads);
+    unsigned seen[R::STAGES];           // of the stages under way, the next to be read first
+#pragma unroll
+    for (int i = 0; i < R::STAGES - 1; ++i) seen[i] = issue_next(i);
+    Warp::split_queries(loaded, query, q_unit);
+    __syncthreads();
+    int at = 0, to = R::STAGES - 1;
+    for (;;) {
+        Warp mine_;
+        mine_.begin(p, q_unit);
+        for (int n = 0; n < piece.tiles; ++n) {
+            copies_wait<R::STAGES - 2>();
+            __syncwarp();               // this stage has landed for all lanes, and all are done with the one before it
+            seen[R::STAGES - 1] = issue_next(to);
+            mine_.step(ring + at * R::STAGE, seen[0], query);
+#pragma unroll
+            for (int i = 0; i + 1 < R::STAGES; ++i) seen[i] = seen[i + 1];
+            at = at + 1 == R::STAGES ? 0 : at + 1;
+            to = to + 1 == R::STAGES ? 0 : to + 1;
         }
+        Piece next = piece;
+        const bool more = behind.next(range_of, tiles_of_heads, TILE, next);
+        const Heads next_heads = heads_of<HEADS>(p, next.head_tile);
+        if (more) Warp::load_queries(loaded, p, next.row, next_heads);
+        mine_.finish();
+        __syncwarp();
+        // no copy is under way into the stage read last, which is the next to be filled
+        auto sums = [&](int j, int h, int c) { return reinterpret_cast<float*>(rings + j * R::BYTES + to * R::STAGE) + h * DP + c; };
+        mine_.put(sums(warp, 0, 0), ml[warp]);
         __syncthreads();
         // ---- the four warps' sums into the result, or into the workspace when the segment is shared with other workers
-        const bool whole = unit == seg_begin && stop == seg_end;
-        const int slot = part_slot(w, unit == seg_begin);
-        for (int i = tid; i < s.heads * (p.d / 4); i += THREADS) {
+        const bool whole = piece.begins && piece.ends;
+        const int slot = part_slot(w, piece.begins);
+        for (int i = tid; i < heads.count * (p.d / 4); i += THREADS) {
             const int h = i / (p.d / 4), c = i % (p.d / 4) * 4;
             float m = ml[0][h].x;
 #pragma unroll
@@ -948,17 +951,21 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
             }
             if (whole) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                float* o = p.o + s.row * p.os[0] + (s.head0 + h) * p.os[1] + c;
+                float* o = p.o + piece.row * p.os[0] + (heads.head0 + h) * p.os[1] + c;
                 o[0] = a.x * inv; o[1] = a.y * inv; o[2] = a.z * inv; o[3] = a.w * inv;
-                if (p.lse && c == 0) p.lse[(int64_t)s.row * p.q_heads + s.head0 + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+                if (p.lse && c == 0) p.lse[(int64_t)piece.row * p.q_heads + heads.head0 + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
             } else {
                 *reinterpret_cast<float4*>(p.part_acc + ((int64_t)slot * HEADS + h) * p.d + c) = a;
                 if (c == 0) p.part_ml[slot * HEADS + h] = make_float2(m, l);
             }
         }
-        if (tid == 0 && unit == seg_begin && stop < seg_end) p.joins[w] = make_int4(s.row, ht, worker_of(units, workers, seg_end - 1), 1);
+        if (tid == 0 && piece.begins && !piece.ends)
+            p.joins[w] = make_int4(piece.row, piece.head_tile, worker_of(units, workers, piece.segment_end - 1), 1);
+        if (!more) return;
+        Warp::split_queries(loaded, query, q_unit);
         __syncthreads();
-        unit = stop;
+        piece = next;
+        heads = next_heads;
     }
 }
 

@@ -2,9 +2,10 @@
 // plain C++, by the host-side tests.
 //
 // A segment is one (row, head tile): a row's keys and values read by the query heads of one tile.  It consists of tiles of
-// `tile` consecutive positions on the absolute grid (so that a tile of aligned pages starts at a page's multiple of 16).
-// All segments' tiles are numbered row by row, head tile by head tile; worker w of W takes the units
-// [U w / W, U (w + 1) / W) of the U (W <= U: every worker has one): equal shares whatever the lengths, at most one unfinished segment at either end.
+// `tile` consecutive positions on the absolute grid (so that 16 tokens from a multiple of 16 are never cut), and counts as
+// that many units and SEGMENT_COST more for its beginning and end.  All segments' units are numbered row by row, head tile
+// by head tile; worker w of W takes the units [U w / W, U (w + 1) / W) of the U (W <= U: every worker has one): equal
+// shares whatever the lengths, at most one unfinished segment at either end.
 #pragma once
 #include "kv_place.h"
 
@@ -28,8 +29,79 @@ TE_HD int64_t worker_begin(int64_t units, int workers, int w) { return units * w
 // The worker whose share holds unit u: the smallest w with worker_begin(w + 1) > u.
 TE_HD int worker_of(int64_t units, int workers, int64_t u) { return (int)(((u + 1) * workers + units - 1) / units) - 1; }
 
+constexpr int SEGMENT_COST = 1;
+// Units of a row's segment; a row without tiles has none.
+TE_HD int segment_units(int tiles) { return tiles > 0 ? tiles + SEGMENT_COST : 0; }
+
 // Where a worker keeps the part of a segment that it does not finish alone: place 0 for the segment its share begins
 // inside of, place 1 for the one that begins in its share and continues behind it.
 TE_HD int part_slot(int worker, bool begins_here) { return 2 * worker + (begins_here ? 1 : 0); }
+
+// What a worker computes of one segment.
+struct Piece {
+    int row, head_tile;
+    RowRange range;
+    int64_t first_tile;        // on the absolute grid
+    int tiles;
+    bool begins, ends;         // holds the segment's first tile, its last
+    int64_t segment_end;       // unit behind the segment
+};
+
+// Goes through a worker's pieces in order.  RangeOf: row -> RowRange.
+struct Walker {
+    int64_t unit, end;         // of the share: what is left
+    int64_t segment;           // first unit of the present segment
+    int row, head_tile, tiles; // tiles of the present row, -1 before it has been looked at
+    RowRange range;
+
+    // The share [unit, end) begins in row `row`, whose units begin at row_begin.
+    TE_HD void start(int64_t unit_, int64_t end_, int row_, int64_t row_begin) {
+        unit = unit_;
+        end = end_;
+        segment = row_begin;
+        row = row_;
+        head_tile = 0;
+        tiles = -1;
+        range.first = range.n = 0;
+    }
+    template <class RangeOf>
+    TE_HD bool next(const RangeOf& range_of, int head_tiles, int tile, Piece& piece) {
+        while (unit < end) {
+            if (tiles < 0) {
+                range = range_of(row);
+                tiles = row_tiles(range, tile);
+                if (tiles > 0 && unit - segment >= segment_units(tiles)) {      // only in the share's first row
+                    const int64_t skip = (unit - segment) / segment_units(tiles);
+                    head_tile = (int)skip;
+                    segment += skip * segment_units(tiles);
+                }
+            }
+            if (tiles == 0 || head_tile >= head_tiles) {
+                ++row;
+                head_tile = 0;
+                tiles = -1;
+                continue;
+            }
+            const int64_t segment_end = segment + segment_units(tiles), stop = end < segment_end ? end : segment_end;
+            const int64_t a = unit - segment - SEGMENT_COST, b = stop - segment - SEGMENT_COST;
+            const int from = a > 0 ? (int)a : 0, to = b > 0 ? (int)b : 0;
+            piece.row = row;
+            piece.head_tile = head_tile;
+            piece.range = range;
+            piece.first_tile = range.first / tile + from;
+            piece.tiles = to - from;
+            piece.begins = from == 0;
+            piece.ends = to == tiles;
+            piece.segment_end = segment_end;
+            unit = stop;
+            if (stop == segment_end) {
+                segment = segment_end;
+                ++head_tile;
+            }
+            if (to > from) return true;
+        }
+        return false;
+    }
+};
 
 }  // namespace te
