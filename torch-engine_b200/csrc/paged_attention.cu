@@ -38,6 +38,9 @@ constexpr int THREADS = 32 * WARPS;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
+// Thread blocks per SM
+constexpr int blocks_per_sm(int dtype, int d) { return dtype == TE_KV_E4M3 ? (d <= 128 ? 3 : 2) : d <= 128 ? (dtype == TE_KV_BF16 ? 3 : 2) : 1; }
+
 struct AttnParams {
     const float* q;
     float* o;
@@ -316,14 +319,14 @@ struct TensorWarp {
     static constexpr int ES = E4M3 ? 1 : 2;
     static constexpr int TOKENS = DP * ES <= 128 ? 32 : 16;             // 8 KB a stage (16 for bf16 rows of 256)
     static constexpr int NK = TOKENS / 16;
-    typedef Ring<DP, ES, TOKENS, 3, E4M3, PACKED> R;
+    static constexpr int BLOCKS = blocks_per_sm(DTYPE, DP);
+    typedef Ring<DP, ES, TOKENS, BLOCKS == 3 ? 2 : 3, E4M3, PACKED> R;
     static constexpr int KG = E4M3 ? DP / 64 : DP / 32;                 // groups of 4 lanes x 16 bytes of a key
     static constexpr int VW = E4M3 && DP < 128 ? 8 : 16;                // bytes of a value a lane holds per chunk
     static constexpr int VE = VW / ES;                                  // elements of it
     static constexpr int VC = DP / (8 * VE);                            // chunks of 8 lanes
     static constexpr int KQ = THREE ? 2 : 4;                            // left operands of Q per group, 16 bytes a lane each
     static constexpr int Q_BYTES = KG * KQ * 32 * 16;
-    static constexpr int MIN_BLOCKS = R::BYTES * WARPS > 110000 ? 1 : 2;
     static constexpr float LIFT = 10.0f;        // e4m3: weights reach 2^10, so that the lower of their two half terms keeps 2^-34 of the largest
 
     static constexpr int QH = HEADS / WARPS, QP = DP / 64;               // heads a warp splits, pairs of elements a lane
@@ -613,7 +616,8 @@ template <int DP, int HT, bool PACKED>
 struct FmaWarp {
     static constexpr int HEADS = HT;
     static constexpr int TOKENS = DP <= 64 ? 16 : 8;
-    typedef Ring<DP, 4, TOKENS, 3, false, PACKED> R;
+    static constexpr int BLOCKS = blocks_per_sm(TE_KV_F32, DP);
+    typedef Ring<DP, 4, TOKENS, BLOCKS == 3 ? 2 : 3, false, PACKED> R;
     static constexpr int TG = TOKENS / 8;                  // tokens whose keys a lane takes parts of
     static constexpr int KC = DP / 16;                     // 16-byte pieces of a key a lane takes
     static constexpr int LPT = DP / 4 < 32 ? DP / 4 : 32;  // lanes along a value
@@ -623,7 +627,6 @@ struct FmaWarp {
     static constexpr int OWN = (HT + 3) / 4;               // heads whose weights a lane computes
     static constexpr int Q_BYTES = HT * DP * 4 + WARPS * (TOKENS * HT + HT) * 8;     // queries, then each warp's weights and factors,
                                                                                      // doubled for two FMAs at once
-    static constexpr int MIN_BLOCKS = R::BYTES * WARPS > 110000 ? 1 : 2;
 
     static constexpr int QN = (HT * DP + THREADS - 1) / THREADS;
 
@@ -798,7 +801,7 @@ template <int DP, int HT, bool PACKED> struct WarpOf<TE_KV_F32, DP, HT, PACKED> 
 
 // ---------------------------------------------------------------------------------------------------- the two kernels
 template <int DTYPE, int DP, int HT, bool PACKED>
-__global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::MIN_BLOCKS) paged_attention_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::BLOCKS) paged_attention_kernel(const AttnParams p) {
     typedef typename WarpOf<DTYPE, DP, HT, PACKED>::type Warp;
     typedef typename Warp::R R;
     constexpr int HEADS = Warp::HEADS, TILE = R::STEP;
@@ -1035,12 +1038,9 @@ int heads_per_tile(int dtype, int64_t group) {
     return dtype == TE_KV_BF16 || group >= 3 ? 4 : (int)group;
 }
 
-// Thread blocks per SM: two where two rings fit the shared memory, one for the longest rows.
-int blocks_per_sm(int dtype, int64_t d) { return dtype == TE_KV_E4M3 || d <= 128 ? 2 : 1; }
-
 size_t workspace_need(const te_paged_attn_desc* t, int sm_count) {
     if (t->rows == 0 || t->q_heads == 0) return 0;
-    const size_t workers = (size_t)sm_count * blocks_per_sm(t->cache.dtype, t->cache.d), heads = heads_per_tile(t->cache.dtype, t->q_heads / t->cache.heads);
+    const size_t workers = (size_t)sm_count * blocks_per_sm(t->cache.dtype, (int)t->cache.d), heads = heads_per_tile(t->cache.dtype, t->q_heads / t->cache.heads);
     return workers * 16 + 2 * workers * heads * (8 + 4 * (size_t)t->cache.d);
 }
 
@@ -1121,7 +1121,7 @@ int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* t, te_st
         snprintf(msg, sizeof msg, "context workspace (%zu bytes) too small; paged attention needs %zu bytes", ctx->workspace_bytes, need);
         return fail(TE_ERR_WORKSPACE, msg);
     }
-    const int workers = ctx->sm_count * blocks_per_sm(c.dtype, c.d);
+    const int workers = ctx->sm_count * blocks_per_sm(c.dtype, (int)c.d);
     AttnParams p;
     p.q = t->q; p.o = t->o; p.lse = t->lse;
     p.kc = static_cast<const char*>(c.k); p.vc = static_cast<const char*>(c.v); p.k_scale = c.k_scale; p.v_scale = c.v_scale;
