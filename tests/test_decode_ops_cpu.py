@@ -36,6 +36,32 @@ int main(void) {
     assert rows == [(C.sizeof(m), getattr(m, f).offset) for m, f in mirrors]
 
 
+def test_packed_descriptors_are_the_structures():
+    """The struct.pack forms put every field where the ctypes mirrors (and so the header) have it."""
+    def fill(desc, start):
+        values, n = [], start
+        for name, kind in desc._fields_:
+            if issubclass(kind, C.Structure):
+                inner, n = fill(getattr(desc, name), n)
+                values += inner
+            elif issubclass(kind, C.Array):
+                setattr(desc, name, kind(*range(n, n + kind._length_)))
+                values += range(n, n + kind._length_)
+                n += kind._length_
+            else:
+                setattr(desc, name, n)
+                values.append(n)
+                n += 1
+        return values, n
+    cache_values = fill(L.KvCacheDesc(), 1)[0]
+    for desc, pack in ((L.RotaryDesc(), L.ROTARY_PACK), (L.KvCacheDesc(), L.KV_CACHE_PACK)):
+        assert pack.pack(*fill(desc, 1)[0]) == bytes(desc)
+    for desc, pack in ((L.KvDesc(), L.KV_PACK), (L.PagedAttnDesc(), L.PAGED_ATTN_PACK)):
+        values = fill(desc, 1)[0]
+        n = len(cache_values)
+        assert L.KV_CACHE_PACK.pack(*values[:n]) + pack.pack(*values[n:]) == bytes(desc)
+
+
 @pytest.mark.parametrize("rot,base", [(0, 10000.0), (2, 10000.0), (64, 10000.0), (128, 500000.0), (34, 100.0)])
 def test_frequencies(rot, base):
     """Against the formulas in Python floats: pow and the few products of either side are within some ulps of 2^-53."""

@@ -4,6 +4,7 @@ Loading fails loudly when libte_b200.so has not been built: there is no Python o
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libte_b200.so")
@@ -122,6 +123,13 @@ class PagedAttnDesc(C.Structure):
     ]
 
 
+# The same four as one struct.pack each, in the order of the fields: filling a Structure field by field takes ten times as
+# long, which a call for a single token feels.  KV_CACHE goes in front of the two that begin with a cache.
+ROTARY_PACK = struct.Struct("@5qP3qP3qP2qPf3i")
+KV_CACHE_PACK = struct.Struct("@4qP3qP3q2P3q2i")
+KV_PACK = struct.Struct("@2qP3qP3qP2qP2q")
+PAGED_ATTN_PACK = struct.Struct("@2qP2qP2q2P2qPqfi")
+
 # name -> (restype, argtypes); every symbol include/te_b200.h declares
 SIGNATURES = {
     "te_b200_init": (C.c_int, [C.c_int, C.c_size_t, C.POINTER(C.c_void_p)]),
@@ -164,10 +172,10 @@ SIGNATURES = {
     "te_b200_cross_entropy": (C.c_int, [C.c_void_p] + [C.c_void_p] * 4 + [C.c_float, C.c_int64, C.c_int64, C.c_void_p]),
     "te_b200_rotary_inv_freq": (C.c_int, [C.c_int64, C.c_double, C.c_int, C.c_double, C.c_int64, C.c_double, C.c_double,
                                           C.POINTER(C.c_double)]),
-    "te_b200_rotary": (C.c_int, [C.c_void_p, C.POINTER(RotaryDesc), C.c_void_p]),
-    "te_b200_kv_append": (C.c_int, [C.c_void_p, C.POINTER(KvDesc), C.c_void_p]),
-    "te_b200_kv_read": (C.c_int, [C.c_void_p, C.POINTER(KvDesc), C.c_void_p]),
-    "te_b200_paged_attention": (C.c_int, [C.c_void_p, C.POINTER(PagedAttnDesc), C.c_void_p]),
+    "te_b200_rotary": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "te_b200_kv_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "te_b200_kv_read": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "te_b200_paged_attention": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "te_b200_paged_attention_workspace_size": (C.c_int, [C.POINTER(PagedAttnDesc), C.c_int, C.POINTER(C.c_size_t)]),
     "te_b200_comm_unique_id": (C.c_int, [C.c_void_p]),
     "te_b200_comm_init": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(C.c_void_p)]),

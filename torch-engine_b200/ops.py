@@ -42,10 +42,6 @@ _KV_NAMES = {"f32": torch.float32, "bf16": torch.bfloat16, "e4m3": torch.float8_
 _ROTARY_SCALINGS = {None: L.TE_ROTARY_PLAIN, "linear": L.TE_ROTARY_LINEAR, "base": L.TE_ROTARY_BASE, "parts": L.TE_ROTARY_PARTS}
 
 
-def _strides(t, n):
-    return (C.c_int64 * n)(*t.stride()[:n])
-
-
 def _i64(seq):
     n = max(len(seq), 1)
     return (C.c_int64 * n)(*seq)
@@ -77,14 +73,9 @@ class KvCache:
                 raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, "KvCache: the last dimension must have unit stride")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.heads, self.page_size, self.d = k.shape
-        c = L.KvCacheDesc()
-        c.pages, c.heads, c.page_size, c.d = k.shape
-        c.k, c.v = k.data_ptr(), v.data_ptr()
-        c.k_strides, c.v_strides = _strides(k, 3), _strides(v, 3)
-        if eight_bit:
-            c.k_scale, c.v_scale, c.scale_strides = k_scale.data_ptr(), v_scale.data_ptr(), _strides(k_scale, 3)
-        c.dtype = _KV_DTYPES[k.dtype]
-        self.desc = c
+        scales = (k_scale.data_ptr(), v_scale.data_ptr()) + k_scale.stride() if eight_bit else (0, 0, 0, 0, 0)
+        self.desc = L.KV_CACHE_PACK.pack(*k.shape, k.data_ptr(), *k.stride()[:3], v.data_ptr(), *v.stride()[:3], *scales,
+                                         _KV_DTYPES[k.dtype], 0)      # struct te_kv_cache
 
 
 class Backend:
@@ -112,7 +103,8 @@ class Backend:
 
     # ------------------------------------------------------------------ helpers
     def _stream(self):
-        return C.c_void_p(torch.cuda.current_stream(self.torch_device).cuda_stream)
+        # the handle of torch.cuda.current_stream(device) without building the Stream object (2 us a call)
+        return C.c_void_p(torch._C._cuda_getCurrentRawStream(self.device))
 
     def _check_f32_cuda(self, *ts):
         for t in ts:
@@ -413,7 +405,7 @@ class Backend:
     # ------------------------------------------------------------------ answering token by token
     def _check_here(self, who, dtype, *ts):
         for t in ts:
-            if t.dtype != dtype or t.device != self.torch_device:
+            if t.dtype is not dtype or t.get_device() != self.device:
                 raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "%s: expected %s tensors on %s" % (who, dtype, self.torch_device))
 
     def rotary_inv_freq(self, rot, base=10000.0, scaling=None, factor=1.0, trained_length=0, slow_turns=1.0, fast_turns=32.0):
@@ -441,26 +433,29 @@ class Backend:
         self._check_here("rotary", torch.float64, inv_freq)
         if x.dim() != 4:
             raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "rotary expects a [B,H,T,d] view")
-        B, H, T, dim = x.shape
-        shared = positions.dim() == 1
-        if tuple(positions.shape) != ((T,) if shared else (B, T)) or inv_freq.dim() != 1:
+        shape = x.shape
+        B, H, T, dim = shape
+        at = positions.shape
+        if (at != (B, T) and at != (T,)) or inv_freq.dim() != 1:
             raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "rotary expects positions [B,T] or [T] and one-dimensional frequencies")
         if out is None:
-            out = torch.empty((B, H, T, dim), dtype=torch.float32, device=x.device)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         else:
             self._check_here("rotary", torch.float32, out)
-            if out.shape != x.shape:
+            if out.shape != shape:
                 raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "rotary: out must be shaped like x")
-        if dim > 1 and (x.stride(3) != 1 or out.stride(3) != 1):
+        xs, ys, ps = x.stride(), out.stride(), positions.stride()
+        if dim > 1 and (xs[3] != 1 or ys[3] != 1):
             raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, "rotary: the last dimension must have unit stride")
-        d = L.RotaryDesc()
-        d.B, d.H, d.T, d.d, d.rot = B, H, T, dim, 2 * inv_freq.numel()
-        d.x, d.x_strides, d.y, d.y_strides = x.data_ptr(), _strides(x, 3), out.data_ptr(), _strides(out, 3)
-        d.positions = positions.data_ptr()
-        d.position_strides = (C.c_int64 * 2)(0, positions.stride(0)) if shared else _strides(positions, 2)
-        d.inv_freq = (inv_freq if inv_freq.is_contiguous() else inv_freq.contiguous()).data_ptr()
-        d.scale, d.interleaved, d.inverse = scale, int(bool(interleaved)), inverse
-        L.check(self._lib.te_b200_rotary(self._ctx, C.byref(d), self._stream()))
+        if not inv_freq.is_contiguous():
+            inv_freq = inv_freq.contiguous()
+        if len(ps) == 1:
+            ps = (0, ps[0])
+        d = L.ROTARY_PACK.pack(B, H, T, dim, 2 * inv_freq.shape[0], x.data_ptr(), xs[0], xs[1], xs[2], out.data_ptr(), ys[0], ys[1], ys[2],
+                               positions.data_ptr(), ps[0], ps[1], inv_freq.data_ptr(), scale, 1 if interleaved else 0, inverse, 0)
+        status = self._lib.te_b200_rotary(self._ctx, d, self._stream())
+        if status:
+            L.check(status)
         return out
 
     def kv_cache(self, pages, heads, page_size, d, dtype="f32"):
@@ -472,41 +467,41 @@ class Backend:
         scales = [torch.ones((pages, heads, page_size), device=self.torch_device) for _ in range(2)] if dtype == "e4m3" else (None, None)
         return KvCache(k, v, *scales)
 
-    def _kv_desc(self, who, cache, page_table, positions):
+    def _kv_move(self, who, entry, cache, k, v, page_table, positions):
+        at, table = positions.shape, page_table.shape
+        if len(table) != 2 or len(at) != 2 or table[0] != at[0]:
+            raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, who + " expects page_table [B, pages] and positions [B,T]")
         self._check_here(who, torch.int64, page_table, positions)
         self._check_here(who, cache.k.dtype, cache.k)
-        if page_table.dim() != 2 or positions.dim() != 2 or page_table.shape[0] != positions.shape[0]:
-            raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, who + " expects page_table [B, pages] and positions [B,T]")
-        if page_table.shape[1] > 1 and page_table.stride(1) != 1:
+        ts, ps = page_table.stride(), positions.stride()
+        if table[1] > 1 and ts[1] != 1:
             raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, who + ": rows of the page table must be contiguous")
-        d = L.KvDesc()
-        d.cache = cache.desc
-        d.B, d.T = positions.shape
-        d.page_table, d.page_table_stride, d.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
-        d.positions, d.position_strides = positions.data_ptr(), _strides(positions, 2)
-        return d
+        shape = (at[0], cache.heads, at[1], cache.d)
+        if k is None:
+            k, v = (torch.empty(shape, dtype=torch.float32, device=self.torch_device) for _ in range(2))
+        elif k.shape != shape or v.shape != shape:
+            raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, who + " expects k and v [B, heads, T, d] as the cache and the positions have them")
+        else:
+            self._check_here(who, torch.float32, k, v)
+        ks, vs = k.stride(), v.stride()
+        if ks[3] != 1 or vs[3] != 1:
+            raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, who + ": the last dimension must have unit stride")
+        d = cache.desc + L.KV_PACK.pack(at[0], at[1], k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
+                                        page_table.data_ptr(), ts[0], table[1], positions.data_ptr(), ps[0], ps[1])
+        status = entry(self._ctx, d, self._stream())
+        if status:
+            L.check(status)
+        return k, v
 
     def kv_append(self, cache, k, v, page_table, positions):
         """Writes k, v [B,H,T,d] (views with a unit last stride) into the cache: token (b, t) at positions[b, t] of sequence b,
         in the page that page_table[b, position // page_size] names.  Negative positions are padding.  The places must
         be distinct; those beyond the table or the cache are skipped and reported by check_device_status."""
-        d = self._kv_desc("kv_append", cache, page_table, positions)
-        self._check_here("kv_append", torch.float32, k, v)
-        for t in (k, v):
-            if tuple(t.shape) != (d.B, cache.heads, d.T, cache.d):
-                raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "kv_append expects k and v [B, heads, T, d] as the cache and the positions have them")
-            if t.stride(3) != 1:
-                raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, "kv_append: the last dimension must have unit stride")
-        d.k, d.k_strides, d.v, d.v_strides = k.data_ptr(), _strides(k, 3), v.data_ptr(), _strides(v, 3)
-        L.check(self._lib.te_b200_kv_append(self._ctx, C.byref(d), self._stream()))
+        self._kv_move("kv_append", self._lib.te_b200_kv_append, cache, k, v, page_table, positions)
 
     def kv_read(self, cache, page_table, positions):
         """(k, v) float32 [B,H,T,d] of the tokens at these positions, addressed as kv_append does; zeros at negative ones."""
-        d = self._kv_desc("kv_read", cache, page_table, positions)
-        k, v = (torch.empty((d.B, cache.heads, d.T, cache.d), dtype=torch.float32, device=self.torch_device) for _ in range(2))
-        d.k, d.k_strides, d.v, d.v_strides = k.data_ptr(), _strides(k, 3), v.data_ptr(), _strides(v, 3)
-        L.check(self._lib.te_b200_kv_read(self._ctx, C.byref(d), self._stream()))
-        return k, v
+        return self._kv_move("kv_read", self._lib.te_b200_kv_read, cache, None, None, page_table, positions)
 
     def paged_attention(self, q, cache, page_table, lens, scale=None, window=0, want_lse=False, out=None):
         """Attention of one new token per row: q [rows, q_heads, d] over the first lens[row] cached tokens of the row's
@@ -517,29 +512,28 @@ class Backend:
         self._check_here(who, torch.float32, q)
         self._check_here(who, torch.int64, page_table, lens)
         self._check_here(who, cache.k.dtype, cache.k)
-        if q.dim() != 3 or q.shape[2] != cache.d:
+        shape, table = q.shape, page_table.shape
+        if len(shape) != 3 or shape[2] != cache.d:
             raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "paged_attention expects q [rows, q_heads, d] with the cache's d")
-        rows, heads, dim = q.shape
-        if page_table.dim() != 2 or page_table.shape[0] != rows or tuple(lens.shape) != (rows,):
+        rows, heads, dim = shape
+        if len(table) != 2 or table[0] != rows or lens.shape != (rows,):
             raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "paged_attention expects page_table [rows, pages] and lens [rows]")
         if out is None:
-            out = torch.empty((rows, heads, dim), dtype=torch.float32, device=q.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             self._check_here(who, torch.float32, out)
-            if out.shape != q.shape:
+            if out.shape != shape:
                 raise L.BackendError(L.TE_ERR_BAD_ARGUMENT, "paged_attention: out must be shaped like q")
-        if q.stride(2) != 1 or out.stride(2) != 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1) or (rows > 1 and lens.stride(0) != 1):
+        qs, os_, ts = q.stride(), out.stride(), page_table.stride()
+        if qs[2] != 1 or os_[2] != 1 or (table[1] > 1 and ts[1] != 1) or (rows > 1 and lens.stride(0) != 1):
             raise L.BackendError(L.TE_ERR_UNSUPPORTED_LAYOUT, "paged_attention: last dimensions must have unit stride")
-        lse = torch.empty((rows, heads), dtype=torch.float32, device=q.device) if want_lse else None
-        d = L.PagedAttnDesc()
-        d.cache = cache.desc
-        d.rows, d.q_heads = rows, heads
-        d.q, d.q_strides, d.o, d.o_strides = q.data_ptr(), _strides(q, 2), out.data_ptr(), _strides(out, 2)
-        d.lse = lse.data_ptr() if want_lse else None
-        d.page_table, d.page_table_stride, d.max_pages = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
-        d.lens = lens.data_ptr()
-        d.window, d.scale = window, dim ** -0.5 if scale is None else scale
-        L.check(self._lib.te_b200_paged_attention(self._ctx, C.byref(d), self._stream()))
+        lse = q.new_empty((rows, heads)) if want_lse else None
+        d = cache.desc + L.PAGED_ATTN_PACK.pack(rows, heads, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os_[0], os_[1],
+                                                lse.data_ptr() if want_lse else 0, page_table.data_ptr(), ts[0], table[1], lens.data_ptr(),
+                                                window, dim ** -0.5 if scale is None else scale, 0)
+        status = self._lib.te_b200_paged_attention(self._ctx, d, self._stream())
+        if status:
+            L.check(status)
         return (out, lse) if want_lse else out
 
     # ------------------------------------------------------------------ row / elementwise ops
