@@ -61,6 +61,8 @@ struct AttnParams {
     float* part_acc;              // [2 * workers][heads of a tile][d]
     float2* part_ml;              // [2 * workers][heads of a tile]: running maximum (base 2) and sum
     int4* joins;                  // [workers]: row, head tile, last worker, 1 -- of the segment that begins in this share and is split
+    int* arrived;                 // [workers] counters, zero between launches: parts done of the segment that begins in a share; NULL
+                                  // where paged_join_kernel adds the parts
     int* status;
 };
 
@@ -800,6 +802,14 @@ template <int DTYPE, int DP, int HT, bool PACKED> struct WarpOf { typedef Tensor
 template <int DP, int HT, bool PACKED> struct WarpOf<TE_KV_F32, DP, HT, PACKED> { typedef FmaWarp<DP, HT, PACKED> type; };
 
 // ---------------------------------------------------------------------------------------------------- the two kernels
+// Four elements of a head's result, from its sums.
+__device__ __forceinline__ void put_result(const AttnParams& p, int row, int head, int c, const float4& a, float m, float l) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float* o = p.o + row * p.os[0] + head * p.os[1] + c;
+    o[0] = a.x * inv; o[1] = a.y * inv; o[2] = a.z * inv; o[3] = a.w * inv;
+    if (p.lse && c == 0) p.lse[(int64_t)row * p.q_heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
 template <int DTYPE, int DP, int HT, bool PACKED>
 __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::BLOCKS) paged_attention_kernel(const AttnParams p) {
     typedef typename WarpOf<DTYPE, DP, HT, PACKED>::type Warp;
@@ -814,6 +824,7 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     __shared__ int64_t scan[WARPS];
     __shared__ int64_t found_prefix;
     __shared__ int found_row;
+    __shared__ bool last_part;
     griddep_wait();
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const int w = blockIdx.x;
@@ -867,7 +878,7 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
             }
         }
     }
-    if (tid == 0) p.joins[w] = make_int4(0, 0, 0, 0);
+    if (tid == 0 && !p.arrived) p.joins[w] = make_int4(0, 0, 0, 0);
     __syncthreads();
     // rows without tokens
     for (int r = w; r < p.rows; r += gridDim.x) {
@@ -953,17 +964,48 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
                 a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
             }
             if (whole) {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                float* o = p.o + piece.row * p.os[0] + (heads.head0 + h) * p.os[1] + c;
-                o[0] = a.x * inv; o[1] = a.y * inv; o[2] = a.z * inv; o[3] = a.w * inv;
-                if (p.lse && c == 0) p.lse[(int64_t)piece.row * p.q_heads + heads.head0 + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+                put_result(p, piece.row, heads.head0 + h, c, a, m, l);
             } else {
                 *reinterpret_cast<float4*>(p.part_acc + ((int64_t)slot * HEADS + h) * p.d + c) = a;
                 if (c == 0) p.part_ml[slot * HEADS + h] = make_float2(m, l);
             }
         }
-        if (tid == 0 && piece.begins && !piece.ends)
+        if (!whole && p.arrived) {
+            // whoever finishes a segment's last part adds them all, in the order of the tokens
+            const int tiles = row_tiles(piece.range, TILE);
+            const int first = worker_of(units, workers, piece.segment_end - tiles), parts = worker_of(units, workers, piece.segment_end - 1) - first + 1;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                last_part = atomicAdd(p.arrived + first, 1) == parts - 1;
+                if (last_part) p.arrived[first] = 0;
+            }
+            __syncthreads();
+            if (last_part) {
+                __threadfence();
+                for (int i = tid; i < heads.count * (p.d / 4); i += THREADS) {
+                    const int h = i / (p.d / 4), c = i % (p.d / 4) * 4;
+                    auto place = [&](int k) { return (int64_t)part_slot(first + k, k == 0) * HEADS + h; };
+                    float m = -INFINITY;
+#pragma unroll 4
+                    for (int k = 0; k < parts; ++k) m = fmaxf(m, __ldcg(p.part_ml + place(k)).x);
+                    const float base = settled(m);
+                    float l = 0.0f;
+                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                    for (int k = 0; k < parts; ++k) {
+                        const float2 part = __ldcg(p.part_ml + place(k));
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_acc + place(k) * p.d + c));
+                        const float f = exp2_of(part.x - base);
+                        l += f * part.y;
+                        a.x += f * x.x; a.y += f * x.y; a.z += f * x.z; a.w += f * x.w;
+                    }
+                    put_result(p, piece.row, heads.head0 + h, c, a, m, l);
+                }
+            }
+        } else if (tid == 0 && piece.begins && !piece.ends) {
             p.joins[w] = make_int4(piece.row, piece.head_tile, worker_of(units, workers, piece.segment_end - 1), 1);
+        }
         if (!more) return;
         Warp::split_queries(loaded, query, q_unit);
         __syncthreads();
@@ -1141,13 +1183,24 @@ int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* t, te_st
     p.part_ml = reinterpret_cast<float2*>(ws + (size_t)workers * 16);
     p.part_acc = reinterpret_cast<float*>(ws + (size_t)workers * 16 + (size_t)workers * 2 * heads * 8);
     p.status = ctx->d_status;
+    // Parts of a segment: at most one per tile, and on average workers per segment.  Few are added by the block that
+    // finishes last (64 FP32 rows: FILL us against FILL with the second kernel); many would keep that one block busy (one row,
+    // one key head: FILL against FILL us), so a kernel of their own adds them.
+    const int64_t segments = (int64_t)p.rows * p.kv_heads * p.head_tiles;
+    int64_t parts = (t->max_pages * c.page_size) / 32 + 1;
+    if (parts > workers / segments + 1) parts = workers / segments + 1;
+    static_assert(STATUS_COUNTER_WORDS >= 1024, "a counter per worker");
+    const bool join_inside = parts <= 16 && workers <= STATUS_COUNTER_WORDS;
+    p.arrived = join_inside ? ctx->d_status + STATUS_COUNTER_WORD : nullptr;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = p.d <= 64 ? launch_width<64>(ctx, p, c.dtype, heads, workers, st) : p.d <= 128 ? launch_width<128>(ctx, p, c.dtype, heads, workers, st)
                                                                                   : launch_width<256>(ctx, p, c.dtype, heads, workers, st);
     if (e != cudaSuccess) return cuda_fail(e, "paged_attention_kernel launch");
+    ctx->launches += 1;
+    if (join_inside) return TE_OK;
     e = launch_pdl(paged_join_kernel, dim3((unsigned)workers, (unsigned)heads), dim3(32 * JOIN_WARPS), 0, st, p, heads);
     if (e != cudaSuccess) return cuda_fail(e, "paged_join_kernel launch");
-    ctx->launches += 2;
+    ctx->launches += 1;
     return TE_OK;
 }
 
