@@ -182,7 +182,7 @@ def test_cache_moves_refuse_by_direction():
 @pytest.mark.parametrize("kw,code,text", CACHE_REFUSALS + [
     (dict(rows=-1), BAD, "extents"), (dict(q_heads=3), BAD, "multiple"), (dict(cache__heads=0), BAD, "multiple"), (dict(window=-1), BAD, "window"),
     (dict(scale=float("inf")), BAD, "finite"), (dict(q=None), BAD, "NULL"), (dict(o=None), BAD, "NULL"), (dict(lens=None), BAD, "NULL"),
-    (dict(o_strides=(256, 32)), LAYOUT, "overlap"), (dict(q_strides=(256, -64)), BAD, "negative"), (dict(rows=1 << 31), BAD, "too many")])
+    (dict(o_strides=(256, 32)), LAYOUT, "overlap"), (dict(max_pages=(1 << 27) - 300, q_heads=64), BAD, "too many heads"), (dict(q_strides=(256, -64)), BAD, "negative"), (dict(rows=1 << 31), BAD, "too many")])
 def test_paged_attention_refuses(kw, code, text):
     d = attn_desc(**kw)
     n = C.c_size_t()
@@ -274,28 +274,31 @@ int main() {
     auto rnd = [&](uint64_t n) { x ^= x << 13; x ^= x >> 7; x ^= x << 17; return x % n; };
     for (int trial = 0; trial < 4000; ++trial) {
         const int tile = trial % 2 ? 64 : 32, heads = 1 + (int)rnd(9), rows = 1 + (int)rnd(12), grid = 1 + (int)rnd(trial % 3 ? 300 : 7);
-        const int64_t window = rnd(3) ? 0 : 1 + (int64_t)rnd(500), most = 3000;
-        std::vector<int64_t> len(rows), row_begin(rows + 1, 0);
+        const int64_t window = rnd(3) ? 0 : 1 + (int64_t)rnd(500);
+        const int most = 3000;
+        std::vector<int64_t> len(rows);
+        std::vector<int> row_begin(rows + 1, 0);
         for (int r = 0; r < rows; ++r) {
             len[r] = (int64_t)rnd(8) == 0 ? -(int64_t)rnd(3) : (int64_t)rnd(trial % 5 ? 3500 : 70);
             const RowRange range = row_range(len[r], most, window);
-            bad += range.n != std::max<int64_t>(0, std::min(len[r], most)) || range.first != (window ? std::max<int64_t>(0, range.n - window) : 0);
+            bad += range.n != std::max<int64_t>(0, std::min<int64_t>(len[r], most)) || range.first != (window ? std::max<int64_t>(0, range.n - window) : 0);
             const int c = row_tiles(range, tile);
             if (range.n > range.first) bad += c != (range.n - 1) / tile - range.first / tile + 1; else bad += c != 0;
-            row_begin[r + 1] = row_begin[r] + (int64_t)segment_units(c) * heads;
+            row_begin[r + 1] = row_begin[r] + segment_units(c) * heads;
         }
-        const int64_t units = row_begin[rows];
+        const int units = row_begin[rows];
         if (!units) continue;
         auto range_of = [&](int r) { return row_range(len[r], most, window); };
-        const int workers = (int)std::min<int64_t>(grid, units);
-        bad += worker_begin(units, workers, 0) != 0 || worker_begin(units, workers, workers) != units;
-        std::map<std::pair<int, int>, int64_t> done;                        // (row, head tile) -> tiles covered so far
+        const int workers = std::min(grid, units);
+        const Shares shares = shares_of(units, workers);
+        bad += share_begin(shares, 0) != 0 || share_begin(shares, workers) != units;
+        std::map<std::pair<int, int>, int> done;                            // (row, head tile) -> tiles covered so far
         std::map<int, std::pair<int, int>> place;                           // part slot -> its segment
         std::map<std::pair<int, int>, std::vector<int>> parts;              // segment -> slots in order of its tiles
         std::map<std::pair<int, int>, std::pair<int, int>> join;            // segment -> first and last worker
         for (int w = 0; w < workers; ++w) {
-            const int64_t u0 = worker_begin(units, workers, w), u1 = worker_begin(units, workers, w + 1);
-            bad += u1 <= u0 || worker_of(units, workers, u0) != w || worker_of(units, workers, u1 - 1) != w;
+            const int u0 = share_begin(shares, w), u1 = share_begin(shares, w + 1);
+            bad += u1 <= u0 || u1 - u0 > units / workers + 1 || worker_of(shares, u0) != w || worker_of(shares, u1 - 1) != w;
             int r = 0;
             while (row_begin[r + 1] <= u0) ++r;
             Walker walk;
@@ -311,7 +314,7 @@ int main() {
                 bad += p.begins != (done[seg] == 0);
                 done[seg] += p.tiles;
                 bad += p.ends != (done[seg] == tiles) || done[seg] > tiles;
-                bad += p.segment_end != row_begin[p.row] + (int64_t)(p.head_tile + 1) * segment_units(tiles);
+                bad += p.segment_end != row_begin[p.row] + (p.head_tile + 1) * segment_units(tiles);
                 bad += p.row < last_row || (p.row == last_row && p.head_tile <= last_head);
                 last_row = p.row; last_head = p.head_tile;
                 if (!(p.begins && p.ends)) {
@@ -320,7 +323,7 @@ int main() {
                     place[slot] = seg;
                     parts[seg].push_back(slot);
                 }
-                if (p.begins && !p.ends) join[seg] = std::make_pair(w, worker_of(units, workers, p.segment_end - 1));
+                if (p.begins && !p.ends) join[seg] = std::make_pair(w, worker_of(shares, p.segment_end - 1));
             }
         }
         for (int r = 0; r < rows; ++r)

@@ -54,8 +54,9 @@ struct AttnParams {
     int64_t qs[2], os[2];
     int64_t kcs[3], vcs[3];       // bytes
     int64_t ss[3];                // elements
-    int64_t table_stride, max_pages, pages, window;
+    int64_t table_stride, pages, window;
     FastDivisor page_size;
+    int most;                     // positions the page table reaches
     int rows, q_heads, kv_heads, group, head_tiles, d;
     float scale;
     float* part_acc;              // [2 * workers][heads of a tile][d]
@@ -72,8 +73,8 @@ struct Heads {
 template <int HT>
 __device__ __forceinline__ Heads heads_of(const AttnParams& p, int head_tile) {
     Heads h;
-    h.kv_head = head_tile / p.head_tiles;
-    const int part = head_tile % p.head_tiles * HT;
+    h.kv_head = p.head_tiles == 1 ? head_tile : head_tile / p.head_tiles;
+    const int part = (head_tile - h.kv_head * p.head_tiles) * HT;
     h.head0 = h.kv_head * p.group + part;
     h.count = min(HT, p.group - part);
     return h;
@@ -200,11 +201,11 @@ struct Ring {
     unsigned slot[NB];
 
     // Reads the page table for the tokens from t0 on; lane's own token (!PACKED), or the page of each block.
-    __device__ __forceinline__ void look_up(const AttnParams& p, const int64_t* table, int64_t t0, int64_t n) {
+    __device__ __forceinline__ void look_up(const AttnParams& p, const int64_t* table, int t0, int n) {
         const int lane = threadIdx.x % 32;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const int64_t t = t0 + (PACKED ? b * BLOCK : lane % TOKENS);
+            const int t = t0 + (PACKED ? b * BLOCK : lane % TOKENS);
             entry[b] = -1;
             slot[b] = 0;
             if (t < n) {                               // n is within the table
@@ -217,14 +218,14 @@ struct Ring {
 
     // Issues the copies of the tokens from t0 on, whose places look_up has read, into stage i.  Returns which of them may be
     // attended to: bit t for token t0 + t.
-    __device__ __forceinline__ unsigned issue(const AttnParams& p, const RowRange& range, int kv_head, int64_t t0, int i) {
+    __device__ __forceinline__ unsigned issue(const AttnParams& p, const RowRange& range, int kv_head, int t0, int i) {
         const int lane = threadIdx.x % 32;
         const unsigned to = base + i * STAGE;
         const int chunk = lane % (CPR < 32 ? CPR : 32), sub = CPR >= 32 ? 0 : lane / CPR;
         const char* kc = p.kc + kv_head * p.kcs[1];
         const char* vc = p.vc + kv_head * p.vcs[1];
         // tokens inside the range, then those on pages of the cache
-        const int64_t lo = range.first - t0, hi = range.n - t0;
+        const int lo = range.first - t0, hi = range.n - t0;
         unsigned seen = hi <= 0 ? 0u : hi >= TOKENS ? 0xffffffffu >> (32 - TOKENS) : (1u << hi) - 1u;
         if (lo > 0) seen = lo >= TOKENS ? 0u : seen & ~((1u << lo) - 1u);
         unsigned good = 0u;
@@ -821,54 +822,53 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     static_assert(HEADS * DP * 4 <= R::STAGE, "a warp's sums fit the stage it read last");
     __shared__ float2 ml[WARPS][HEADS];
     __shared__ float q_unit[HEADS];
-    __shared__ int64_t scan[WARPS];
-    __shared__ int64_t found_prefix;
+    __shared__ int scan[WARPS];
+    __shared__ int found_prefix;
     __shared__ int found_row;
     __shared__ bool last_part;
     griddep_wait();
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const int w = blockIdx.x;
     const int tiles_of_heads = p.kv_heads * p.head_tiles;
-    const int64_t most = p.max_pages * (int64_t)p.page_size.divisor;
-
-    auto range_of = [&](int r) { return row_range(p.lens[r], most, p.window); };
+    auto range_of = [&](int r) { return row_range(p.lens[r], p.most, p.window); };
 
     // ---- this worker's share: the rows' units, added up by all threads over slabs of rows
     const int slab = (p.rows + THREADS - 1) / THREADS;
     const int r0 = min(p.rows, tid * slab), r1 = min(p.rows, r0 + slab);
-    int64_t mine = 0;
-    bool cut = false;
+    int mine = 0;
+    bool cut = false, empty = false;
     for (int r = r0; r < r1; ++r) {
         const int64_t len = p.lens[r];
-        cut |= len > most;
-        mine += segment_units(row_tiles(row_range(len, most, p.window), TILE));
+        cut |= len > p.most;
+        const int c = segment_units(row_tiles(row_range(len, p.most, p.window), TILE));
+        empty |= c == 0;
+        mine += c;
     }
     if (cut) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
-    int64_t before = mine;
+    int before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+        const int x = __shfl_up_sync(0xffffffffu, before, o);
         if (lane >= o) before += x;
     }
     if (lane == 31) scan[warp] = before;
-    if (tid == 0) found_row = -1;
-    __syncthreads();
-    int64_t total = 0;
+    empty = __syncthreads_or(empty);
+    int total = 0;
     before -= mine;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) {
         if (i < warp) before += scan[i];
         total += scan[i];
     }
-    const int64_t units = total * tiles_of_heads;
-    const int workers = (int)(units < gridDim.x ? units : (int64_t)gridDim.x);      // every one of them has a unit
-    const int64_t unit = w < workers ? worker_begin(units, workers, w) : 0;
-    const int64_t unit_end = w < workers ? worker_begin(units, workers, w + 1) : 0;
+    const int units = total * tiles_of_heads;
+    const Shares shares = shares_of(units, max(1, min(units, (int)gridDim.x)));       // every worker has a unit
+    const int unit = w < shares.workers ? share_begin(shares, w) : 0;
+    const int unit_end = w < shares.workers ? share_begin(shares, w + 1) : 0;
     if (unit < unit_end) {
-        const int64_t at = unit / tiles_of_heads;          // in the rows' sums
+        const int at = (int)((unsigned)unit / (unsigned)tiles_of_heads);          // in the rows' sums
         if (at >= before && at < before + mine) {
             for (int r = r0; r < r1; ++r) {
-                const int c = segment_units(row_tiles(range_of(r), TILE));
+                const int c = r1 - r0 == 1 ? mine : segment_units(row_tiles(range_of(r), TILE));
                 if (at < before + c) {
                     found_row = r;
                     found_prefix = before;
@@ -880,12 +880,13 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     }
     if (tid == 0 && !p.arrived) p.joins[w] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    // rows without tokens
-    for (int r = w; r < p.rows; r += gridDim.x) {
-        if (row_tiles(range_of(r), TILE) > 0) continue;
-        for (int i = tid; i < p.q_heads * p.d; i += THREADS) p.o[r * p.os[0] + i / p.d * p.os[1] + i % p.d] = 0.0f;
-        if (p.lse)
-            for (int i = tid; i < p.q_heads; i += THREADS) p.lse[(int64_t)r * p.q_heads + i] = -INFINITY;
+    if (empty) {        // some row without tokens
+        for (int r = w; r < p.rows; r += gridDim.x) {
+            if (row_tiles(range_of(r), TILE) > 0) continue;
+            for (int i = tid; i < p.q_heads * p.d; i += THREADS) p.o[r * p.os[0] + i / p.d * p.os[1] + i % p.d] = 0.0f;
+            if (p.lse)
+                for (int i = tid; i < p.q_heads; i += THREADS) p.lse[(int64_t)r * p.q_heads + i] = -INFINITY;
+        }
     }
     if (unit >= unit_end) return;
 
@@ -900,14 +901,18 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     char* ring = rings + warp * R::BYTES;
     R copies;
     copies.base = smem_address(ring);
-    int64_t t0 = soon.first_tile * TILE + warp * R::TOKENS;                  // of this warp's next stage
+    int soon_head = heads_of<HEADS>(p, soon.head_tile).kv_head;
+    int t0 = soon.first_tile * TILE + warp * R::TOKENS;                      // of this warp's next stage
     copies.look_up(p, p.page_table + soon.row * p.table_stride, t0, soon.range.n);
     auto issue_next = [&](int stage) {
         unsigned seen = 0u;
         if (soon.tiles > 0) {
-            seen = copies.issue(p, soon.range, soon.head_tile / p.head_tiles, t0, stage);
+            seen = copies.issue(p, soon.range, soon_head, t0, stage);
             t0 += TILE;
-            if (--soon.tiles == 0 && ahead.next(range_of, tiles_of_heads, TILE, soon)) t0 = soon.first_tile * TILE + warp * R::TOKENS;
+            if (--soon.tiles == 0 && ahead.next(range_of, tiles_of_heads, TILE, soon)) {
+                t0 = soon.first_tile * TILE + warp * R::TOKENS;
+                soon_head = heads_of<HEADS>(p, soon.head_tile).kv_head;
+            }
             if (soon.tiles > 0) copies.look_up(p, p.page_table + soon.row * p.table_stride, t0, soon.range.n);
         }
         copies_issued();
@@ -948,8 +953,9 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
         // ---- the four warps' sums into the result, or into the workspace when the segment is shared with other workers
         const bool whole = piece.begins && piece.ends;
         const int slot = part_slot(w, piece.begins);
-        for (int i = tid; i < heads.count * (p.d / 4); i += THREADS) {
-            const int h = i / (p.d / 4), c = i % (p.d / 4) * 4;
+        for (int i = tid; i < heads.count * (DP / 4); i += THREADS) {
+            const int h = i / (DP / 4), c = i % (DP / 4) * 4;
+            if (c >= p.d) continue;
             float m = ml[0][h].x;
 #pragma unroll
             for (int j = 1; j < WARPS; ++j) m = fmaxf(m, ml[j][h].x);
@@ -973,7 +979,7 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
         if (!whole && p.arrived) {
             // whoever finishes a segment's last part adds them all, in the order of the tokens
             const int tiles = row_tiles(piece.range, TILE);
-            const int first = worker_of(units, workers, piece.segment_end - tiles), parts = worker_of(units, workers, piece.segment_end - 1) - first + 1;
+            const int first = worker_of(shares, piece.segment_end - tiles), parts = worker_of(shares, piece.segment_end - 1) - first + 1;
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -983,8 +989,9 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
             __syncthreads();
             if (last_part) {
                 __threadfence();
-                for (int i = tid; i < heads.count * (p.d / 4); i += THREADS) {
-                    const int h = i / (p.d / 4), c = i % (p.d / 4) * 4;
+                for (int i = tid; i < heads.count * (DP / 4); i += THREADS) {
+                    const int h = i / (DP / 4), c = i % (DP / 4) * 4;
+                    if (c >= p.d) continue;
                     auto place = [&](int k) { return (int64_t)part_slot(first + k, k == 0) * HEADS + h; };
                     float m = -INFINITY;
 #pragma unroll 4
@@ -1004,7 +1011,7 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
                 }
             }
         } else if (tid == 0 && piece.begins && !piece.ends) {
-            p.joins[w] = make_int4(piece.row, piece.head_tile, worker_of(units, workers, piece.segment_end - 1), 1);
+            p.joins[w] = make_int4(piece.row, piece.head_tile, worker_of(shares, piece.segment_end - 1), 1);
         }
         if (!more) return;
         Warp::split_queries(loaded, query, q_unit);
@@ -1016,7 +1023,7 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
 
 // Adds the parts of the segment that begins in worker blockIdx.x's share, in the order of its tokens, for head blockIdx.y of
 // the tile: warps take parts in turn, lanes lie along d; then the warps' sums are added in order.
-constexpr int JOIN_WARPS = 8;
+constexpr int JOIN_WARPS = 16;
 __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(const AttnParams p, int heads_per_tile) {
     __shared__ float sums[JOIN_WARPS][256];
     __shared__ float tops[JOIN_WARPS], totals[JOIN_WARPS];
@@ -1039,7 +1046,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) paged_join_kernel(const AttnP
     for (int i = 1; i < JOIN_WARPS; ++i) m = fmaxf(m, tops[i]);
     const float base = settled(m);
     float a[8] = {}, l = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = warp; i < count; i += JOIN_WARPS) {
         const int64_t o = at(i);
         const float2 ml = p.part_ml[o];
@@ -1123,9 +1130,11 @@ int check_desc(const te_paged_attn_desc* t) {
     if (int bad = check_kv_cache(t->cache, "paged attention")) return bad;
     const te_kv_cache& c = t->cache;
     if (t->q_heads > 0 && (c.heads == 0 || t->q_heads % c.heads)) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: q_heads must be a multiple of the cache's heads");
-    if (t->max_pages > 0 && c.page_size > INT32_MAX / t->max_pages) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: the page table reaches beyond 2^31-1 positions");
+    if (t->max_pages > 0 && c.page_size > (INT32_MAX - 4096) / t->max_pages) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: the page table reaches beyond 2^31-1 positions");
     if (c.pages > INT32_MAX) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: more than 2^31-1 pages");
     if (t->q_heads > 65535 || (t->q_heads > 0 && t->rows > INT32_MAX / t->q_heads)) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: too many rows or heads");
+    if (t->max_pages > 0 && (t->max_pages * c.page_size / 32 + 4) * t->q_heads >= INT32_MAX)
+        return fail(TE_ERR_BAD_ARGUMENT, "paged attention: too many heads for so long a page table");
     if (t->window < 0) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: negative window");
     if (!isfinite(t->scale)) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: scale must be finite");
     if (t->rows == 0 || t->q_heads == 0) return TE_OK;
@@ -1165,15 +1174,14 @@ int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* t, te_st
     }
     const int workers = ctx->sm_count * blocks_per_sm(c.dtype, (int)c.d);
     AttnParams p;
-    p.q = t->q; p.o = t->o; p.lse = t->lse;
     p.kc = static_cast<const char*>(c.k); p.vc = static_cast<const char*>(c.v); p.k_scale = c.k_scale; p.v_scale = c.v_scale;
-    p.page_table = t->page_table; p.lens = t->lens;
     const int64_t size = c.dtype == TE_KV_F32 ? 4 : c.dtype == TE_KV_BF16 ? 2 : 1;
     for (int i = 0; i < 2; ++i) { p.qs[i] = t->q_strides[i]; p.os[i] = t->o_strides[i]; }
     for (int i = 0; i < 3; ++i) { p.kcs[i] = c.k_strides[i] * size; p.vcs[i] = c.v_strides[i] * size; p.ss[i] = c.scale_strides[i]; }
-    p.table_stride = t->page_table_stride; p.max_pages = t->max_pages; p.pages = c.pages; p.window = t->window;
+    p.table_stride = t->page_table_stride; p.pages = c.pages; p.window = t->window;
     p.page_size = make_fast_divisor((uint32_t)c.page_size);
-    p.rows = (int)t->rows; p.q_heads = (int)t->q_heads; p.kv_heads = (int)c.heads;
+    p.most = (int)(t->max_pages * c.page_size);
+    p.q_heads = (int)t->q_heads; p.kv_heads = (int)c.heads;
     p.group = (int)(t->q_heads / c.heads); p.d = (int)c.d;
     const int heads = heads_per_tile(c.dtype, p.group);
     p.head_tiles = (p.group + heads - 1) / heads;
@@ -1183,24 +1191,33 @@ int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* t, te_st
     p.part_ml = reinterpret_cast<float2*>(ws + (size_t)workers * 16);
     p.part_acc = reinterpret_cast<float*>(ws + (size_t)workers * 16 + (size_t)workers * 2 * heads * 8);
     p.status = ctx->d_status;
-    // Parts of a segment: at most one per tile, and on average workers per segment.  Few are added by the block that
-    // finishes last (64 FP32 rows: FILL us against FILL with the second kernel); many would keep that one block busy (one row,
-    // one key head: FILL against FILL us), so a kernel of their own adds them.
-    const int64_t segments = (int64_t)p.rows * p.kv_heads * p.head_tiles;
-    int64_t parts = (t->max_pages * c.page_size) / 32 + 1;
-    if (parts > workers / segments + 1) parts = workers / segments + 1;
-    static_assert(STATUS_COUNTER_WORDS >= 1024, "a counter per worker");
-    const bool join_inside = parts <= 16 && workers <= STATUS_COUNTER_WORDS;
-    p.arrived = join_inside ? ctx->d_status + STATUS_COUNTER_WORD : nullptr;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cudaError_t e = p.d <= 64 ? launch_width<64>(ctx, p, c.dtype, heads, workers, st) : p.d <= 128 ? launch_width<128>(ctx, p, c.dtype, heads, workers, st)
-                                                                                  : launch_width<256>(ctx, p, c.dtype, heads, workers, st);
-    if (e != cudaSuccess) return cuda_fail(e, "paged_attention_kernel launch");
-    ctx->launches += 1;
-    if (join_inside) return TE_OK;
-    e = launch_pdl(paged_join_kernel, dim3((unsigned)workers, (unsigned)heads), dim3(32 * JOIN_WARPS), 0, st, p, heads);
-    if (e != cudaSuccess) return cuda_fail(e, "paged_join_kernel launch");
-    ctx->launches += 1;
+    // so many rows at a time that their units stay below 2^31 (a tile has 32 tokens or more): nearly always all
+    const int64_t row_units = ((int64_t)p.most / 32 + 2 + SEGMENT_COST) * p.kv_heads * p.head_tiles;
+    const int64_t rows_at_once = INT32_MAX / row_units;
+    for (int64_t r = 0; r < t->rows; r += rows_at_once) {
+        p.rows = (int)(t->rows - r < rows_at_once ? t->rows - r : rows_at_once);
+        p.q = t->q + r * t->q_strides[0];
+        p.o = t->o + r * t->o_strides[0];
+        p.lse = t->lse ? t->lse + r * t->q_heads : nullptr;
+        p.page_table = t->page_table + r * t->page_table_stride;
+        p.lens = t->lens + r;
+        // Parts of a segment: at most one per tile, and on average workers per segment.  Few are added by the block that
+        // finishes last; many would keep that one block busy, so a kernel of their own adds them.
+        const int64_t segments = (int64_t)p.rows * p.kv_heads * p.head_tiles;
+        int64_t parts = p.most / 32 + 1;
+        if (parts > workers / segments + 1) parts = workers / segments + 1;
+        const bool join_inside = parts <= 16 && workers <= STATUS_COUNTER_WORDS;
+        p.arrived = join_inside ? ctx->d_status + STATUS_COUNTER_WORD : nullptr;
+        cudaError_t e = p.d <= 64 ? launch_width<64>(ctx, p, c.dtype, heads, workers, st) : p.d <= 128 ? launch_width<128>(ctx, p, c.dtype, heads, workers, st)
+                                                                                      : launch_width<256>(ctx, p, c.dtype, heads, workers, st);
+        if (e != cudaSuccess) return cuda_fail(e, "paged_attention_kernel launch");
+        ctx->launches += 1;
+        if (join_inside) continue;
+        e = launch_pdl(paged_join_kernel, dim3((unsigned)workers, (unsigned)heads), dim3(32 * JOIN_WARPS), 0, st, p, heads);
+        if (e != cudaSuccess) return cuda_fail(e, "paged_join_kernel launch");
+        ctx->launches += 1;
+    }
     return TE_OK;
 }
 
