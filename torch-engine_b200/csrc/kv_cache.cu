@@ -3,9 +3,10 @@
 // cache per element (and 4 B of scale per 8-bit row).
 //
 // A row is the d elements of one (token, head) of k or of v.  A group of LANES lanes holds it, four elements a lane (eight
-// for d > 128), so that FP32 moves in float4s, the largest magnitude of a row is one butterfly within the group, and a
-// row's bytes leave in one coalesced store.  Consecutive groups take consecutive tokens of one head, which lie side by side
-// in the cache's usual order [pages, heads, page_size, d].
+// for d > 128), so that FP32 moves in float4s, the largest magnitude of a row is one reduction within the group, and a
+// row's bytes leave in one coalesced store.  A group moves ROWS consecutive tokens of one head (of k and of v) at once: they lie
+// side by side in the cache's usual order [pages, heads, page_size, d], and their positions, page numbers and data are
+// three loads one after the other that ROWS tokens wait for together.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -30,9 +31,9 @@ struct KvParams {
     const int64_t* positions;
     int64_t ks[3], vs[3], ps[2], kcs[3], vcs[3], ss[3];
     int64_t table_stride, max_pages, pages;
-    int64_t rows;               // B * H * T, T fastest
-    FastDivisor page_size;
-    int T, H, d;
+    FastDivisor page_size, blocks, heads;      // blocks: of ROWS tokens in T
+    int tasks;                                 // B * H * blocks, the last fastest
+    int T, d;
     int* status;
 };
 
@@ -62,23 +63,30 @@ __device__ __forceinline__ void store4(float* p, float4 x) {
     else { p[0] = x.x; p[1] = x.y; p[2] = x.z; p[3] = x.w; }
 }
 
-// Values of one row into the cache at `at`; `x` is this lane's part, element c + 4 * LANES * u + i in x[u] component i.
+// Values of one row into the cache at `row`; `x` is this lane's part, element 4 * (lane + LANES * u) + i in x[u] component i.
 template <int DTYPE, int LANES, int U>
-__device__ __forceinline__ void put_row(const float4 (&x)[U], void* cache, int64_t at, float* scale, int lane, int d, bool there, unsigned mask) {
-    typedef typename Stored<DTYPE>::type S;
-    S* row = static_cast<S*>(cache) + at;
+__device__ __forceinline__ void put_row(const float4 (&x)[U], typename Stored<DTYPE>::type* row, float* scale, int lane, int d, bool there, unsigned mask) {
     float inv = 1.0f;
+    bool finite = true;
     if constexpr (DTYPE == TE_KV_E4M3) {
-        float amax = 0.0f;
+        unsigned top = 0u;             // magnitudes compare like their bits; those of what is not finite come last
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+        for (int u = 0; u < U; ++u)
+            top = max(max(top, max(__float_as_uint(x[u].x) & 0x7fffffffu, __float_as_uint(x[u].y) & 0x7fffffffu)),
+                      max(__float_as_uint(x[u].z) & 0x7fffffffu, __float_as_uint(x[u].w) & 0x7fffffffu));
+        top = __reduce_max_sync(mask, top);
+        finite = top < 0x7f800000u;
+        if (!finite) {                 // (the whole group together)
+            top = 0u;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) amax = fmaxf(amax, is_finite(v[i]) ? fabsf(v[i]) : 0.0f);
+            for (int u = 0; u < U; ++u) {
+                const float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = max(top, is_finite(v[i]) ? __float_as_uint(v[i]) & 0x7fffffffu : 0u);
+            }
+            top = __reduce_max_sync(mask, top);
         }
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
-        const int e = scale_exponent(amax);
+        const int e = scale_exponent(__uint_as_float(top));
         inv = power_of_two(-e);
         if (there && lane == 0) *scale = power_of_two(e);
     }
@@ -97,14 +105,14 @@ __device__ __forceinline__ void put_row(const float4 (&x)[U], void* cache, int64
             *reinterpret_cast<uint2*>(row + c) = w;
         } else {
             // multiplying by the power of two rounds nothing that survives in 8 bits; the conversion rounds to nearest even
-            const float v[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-            unsigned w = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const __nv_fp8_storage_t q = __nv_cvt_float_to_fp8(is_finite(v[i]) ? v[i] * inv : __uint_as_float(0x7fc00000u), __NV_SATFINITE, __NV_E4M3);
-                w |= (unsigned)q << (8 * i);
+            float4 y = x[u];
+            if (!finite) {
+                const float nan = __uint_as_float(0x7fc00000u);
+                y.x = is_finite(y.x) ? y.x : nan; y.y = is_finite(y.y) ? y.y : nan; y.z = is_finite(y.z) ? y.z : nan; y.w = is_finite(y.w) ? y.w : nan;
             }
-            *reinterpret_cast<unsigned*>(row + c) = w;
+            const unsigned lo = __nv_cvt_float2_to_fp8x2(make_float2(y.x * inv, y.y * inv), __NV_SATFINITE, __NV_E4M3);
+            const unsigned hi = __nv_cvt_float2_to_fp8x2(make_float2(y.z * inv, y.w * inv), __NV_SATFINITE, __NV_E4M3);
+            *reinterpret_cast<unsigned*>(row + c) = lo | hi << 16;
         }
     }
 }
@@ -118,92 +126,112 @@ __device__ __forceinline__ float4 get4(const typename Stored<DTYPE>::type* p, fl
         return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
     } else {
         const unsigned w = *reinterpret_cast<const unsigned*>(p);
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(w >> (8 * i)), __NV_E4M3))) * scale;
-        return make_float4(v[0], v[1], v[2], v[3]);
+        const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3)));
+        const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3)));
+        return make_float4(lo.x * scale, lo.y * scale, hi.x * scale, hi.y * scale);
     }
 }
 
-// One group of lanes moves one row of k and the same row of v.
-template <int DTYPE, int LANES, int U, bool VEC, bool APPEND>
+template <int DTYPE, int LANES, int U, int ROWS, bool VEC, bool APPEND>
 __global__ void __launch_bounds__(256) kv_move_kernel(const KvParams p) {
     griddep_wait();
+    typedef typename Stored<DTYPE>::type S;
     constexpr int GROUPS = 256 / LANES;
     const int lane = threadIdx.x % LANES;
-    const int64_t r = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
+    const unsigned task = blockIdx.x * GROUPS + threadIdx.x / LANES;
     const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << (threadIdx.x % 32 / LANES * LANES);
-    if (r >= p.rows) return;                          // the whole group leaves
-    const int64_t bh = r / p.T;
-    const int t = (int)(r - bh * p.T);
-    const int64_t b = bh / p.H;
-    const int h = (int)(bh - b * p.H);
-    float* k = p.k ? p.k + b * p.ks[0] + h * p.ks[1] + t * p.ks[2] : nullptr;
-    float* v = p.v ? p.v + b * p.vs[0] + h * p.vs[1] + t * p.vs[2] : nullptr;
-    const int64_t position = p.positions[b * p.ps[0] + t * p.ps[1]];
+    if (task >= (unsigned)p.tasks) return;            // the whole group leaves
+    const unsigned bh = fast_quotient(task, p.blocks);
+    const int t0 = (int)(task - bh * p.blocks.divisor) * ROWS;
+    const unsigned b = fast_quotient(bh, p.heads);
+    const int h = (int)(bh - b * p.heads.divisor);
+    const int64_t* positions = p.positions + b * p.ps[0];
     const PageRow table = {p.page_table + b * p.table_stride, p.max_pages, p.pages};
+    float* k = p.k + b * p.ks[0] + h * p.ks[1];
+    float* v = p.v + b * p.vs[0] + h * p.vs[1];
+    int64_t position[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) position[i] = t0 + i < p.T ? positions[(t0 + i) * p.ps[1]] : -1;
+    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 x[ROWS][U], y[ROWS][U];
     if constexpr (APPEND) {
-        if (position < 0) return;                     // padding
-        float4 x[U], y[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int c = 4 * (lane + LANES * u);
-            x[u] = c < p.d ? load4<VEC>(k + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-            y[u] = c < p.d ? load4<VEC>(v + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int c = 4 * (lane + LANES * u);
+                const bool in = position[i] >= 0 && c < p.d;       // (nothing is read of padding)
+                x[i][u] = in ? load4<VEC>(k + (t0 + i) * p.ks[2] + c) : zero;
+                y[i][u] = in ? load4<VEC>(v + (t0 + i) * p.vs[2] + c) : zero;
+            }
+    }
+    int64_t page[ROWS];
+    uint32_t slot[ROWS];
+    bool there[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        page[i] = 0;
+        slot[i] = 0u;
+        there[i] = kv_place(table, p.page_size, position[i], page[i], slot[i]);
+        if (!there[i]) {
+            if (position[i] >= 0 && lane == 0) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
+            page[i] = 0;
         }
-        int64_t page = 0;
-        uint32_t slot = 0;
-        const bool there = kv_place(table, p.page_size, position, page, slot);
-        if (!there) {
-            if (lane == 0) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
-            page = 0;
+    }
+    if constexpr (APPEND) {
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int64_t s = DTYPE == TE_KV_E4M3 ? page[i] * p.ss[0] + h * p.ss[1] + slot[i] * p.ss[2] : 0;
+            put_row<DTYPE, LANES, U>(x[i], static_cast<S*>(p.kc) + page[i] * p.kcs[0] + h * p.kcs[1] + slot[i] * p.kcs[2], p.k_scale + s, lane, p.d, there[i], mask);
+            put_row<DTYPE, LANES, U>(y[i], static_cast<S*>(p.vc) + page[i] * p.vcs[0] + h * p.vcs[1] + slot[i] * p.vcs[2], p.v_scale + s, lane, p.d, there[i], mask);
         }
-        const int64_t s = DTYPE == TE_KV_E4M3 ? page * p.ss[0] + h * p.ss[1] + slot * p.ss[2] : 0;
-        put_row<DTYPE, LANES, U>(x, p.kc, page * p.kcs[0] + h * p.kcs[1] + slot * p.kcs[2], p.k_scale + s, lane, p.d, there, mask);
-        put_row<DTYPE, LANES, U>(y, p.vc, page * p.vcs[0] + h * p.vcs[1] + slot * p.vcs[2], p.v_scale + s, lane, p.d, there, mask);
     } else {
-        typedef typename Stored<DTYPE>::type S;
-        int64_t page = 0;
-        uint32_t slot = 0;
-        const bool there = kv_place(table, p.page_size, position, page, slot);
-        if (!there && position >= 0 && lane == 0) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
-        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        float4 x[U], y[U];
-        float sk = 1.0f, sv = 1.0f;
-        if (DTYPE == TE_KV_E4M3 && there) {
-            const int64_t s = page * p.ss[0] + h * p.ss[1] + slot * p.ss[2];
-            if (k) sk = p.k_scale[s];
-            if (v) sv = p.v_scale[s];
-        }
-        const S* kr = static_cast<const S*>(p.kc) + page * p.kcs[0] + h * p.kcs[1] + slot * p.kcs[2];
-        const S* vr = static_cast<const S*>(p.vc) + page * p.vcs[0] + h * p.vcs[1] + slot * p.vcs[2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int c = 4 * (lane + LANES * u);
-            const bool in = there && c < p.d;
-            x[u] = in && k ? get4<DTYPE>(kr + c, sk) : zero;
-            y[u] = in && v ? get4<DTYPE>(vr + c, sv) : zero;
+        for (int i = 0; i < ROWS; ++i) {
+            float sk = 1.0f, sv = 1.0f;
+            if (DTYPE == TE_KV_E4M3 && there[i]) {
+                const int64_t s = page[i] * p.ss[0] + h * p.ss[1] + slot[i] * p.ss[2];
+                if (p.k) sk = p.k_scale[s];
+                if (p.v) sv = p.v_scale[s];
+            }
+            const S* kr = static_cast<const S*>(p.kc) + page[i] * p.kcs[0] + h * p.kcs[1] + slot[i] * p.kcs[2];
+            const S* vr = static_cast<const S*>(p.vc) + page[i] * p.vcs[0] + h * p.vcs[1] + slot[i] * p.vcs[2];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int c = 4 * (lane + LANES * u);
+                const bool in = there[i] && c < p.d;
+                x[i][u] = in && p.k ? get4<DTYPE>(kr + c, sk) : zero;
+                y[i][u] = in && p.v ? get4<DTYPE>(vr + c, sv) : zero;
+            }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int c = 4 * (lane + LANES * u);
-            if (c >= p.d) continue;
-            if (k) store4<VEC>(k + c, x[u]);
-            if (v) store4<VEC>(v + c, y[u]);
+        for (int i = 0; i < ROWS; ++i) {
+            if (t0 + i >= p.T) break;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int c = 4 * (lane + LANES * u);
+                if (c >= p.d) continue;
+                if (p.k) store4<VEC>(k + (t0 + i) * p.ks[2] + c, x[i][u]);
+                if (p.v) store4<VEC>(v + (t0 + i) * p.vs[2] + c, y[i][u]);
+            }
         }
     }
 }
+
+// Tokens a group moves at once: four (two of the longest rows), one where there are few per sequence.
+int rows_at_once(int T, int d) { return T < 4 ? 1 : d > 128 ? 2 : 4; }
 
 template <int DTYPE, bool APPEND>
 cudaError_t launch_move(const KvParams& p, bool vec, cudaStream_t st) {
-    const int lanes = p.d <= 32 ? 8 : p.d <= 64 ? 16 : 32;
-    const int64_t groups = 256 / lanes;
-    const dim3 grid((unsigned)((p.rows + groups - 1) / groups)), block(256);
-#define TE_MOVE(L, U) (vec ? launch_pdl(kv_move_kernel<DTYPE, L, U, true, APPEND>, grid, block, 0, st, p) \
-                           : launch_pdl(kv_move_kernel<DTYPE, L, U, false, APPEND>, grid, block, 0, st, p))
-    if (lanes == 8) return TE_MOVE(8, 1);
-    if (lanes == 16) return TE_MOVE(16, 1);
-    return p.d <= 128 ? TE_MOVE(32, 1) : TE_MOVE(32, 2);
+    const int lanes = p.d <= 32 ? 8 : p.d <= 64 ? 16 : 32, rows = rows_at_once(p.T, p.d);
+    const int groups = 256 / lanes;
+    const dim3 grid((unsigned)((p.tasks + groups - 1) / groups)), block(256);
+#define TE_MOVE(L, U, N) (vec ? launch_pdl(kv_move_kernel<DTYPE, L, U, N, true, APPEND>, grid, block, 0, st, p) \
+                              : launch_pdl(kv_move_kernel<DTYPE, L, U, N, false, APPEND>, grid, block, 0, st, p))
+    if (lanes == 8) return rows == 1 ? TE_MOVE(8, 1, 1) : TE_MOVE(8, 1, 4);
+    if (lanes == 16) return rows == 1 ? TE_MOVE(16, 1, 1) : TE_MOVE(16, 1, 4);
+    if (p.d <= 128) return rows == 1 ? TE_MOVE(32, 1, 1) : TE_MOVE(32, 1, 4);
+    return rows == 1 ? TE_MOVE(32, 2, 1) : TE_MOVE(32, 2, 2);
 #undef TE_MOVE
 }
 
@@ -230,8 +258,7 @@ int move(te_b200_ctx* ctx, const te_kv_desc* t, bool append, cudaStream_t st) {
             if (!append && ext[i] > 1 && ((t->k && t->k_strides[i] < c.d) || (t->v && t->v_strides[i] < c.d)))
                 return fail(TE_ERR_UNSUPPORTED_LAYOUT, name + ": rows of the output overlap");
         }
-        // B, T < 2^31 each: bound their product before the heads come in
-        if ((double)t->B * (double)t->T * (double)c.heads / 8.0 > 2147483647.0) return fail(TE_ERR_BAD_ARGUMENT, name + ": too many rows");
+        if ((double)t->B * (double)t->T * (double)c.heads > 2147483000.0) return fail(TE_ERR_BAD_ARGUMENT, name + ": too many rows");
     }
     if (int bad = check_ctx(ctx)) return bad;
     if (empty) return TE_OK;
@@ -244,9 +271,12 @@ int move(te_b200_ctx* ctx, const te_kv_desc* t, bool append, cudaStream_t st) {
     }
     p.ps[0] = t->position_strides[0]; p.ps[1] = t->position_strides[1];
     p.table_stride = t->page_table_stride; p.max_pages = t->max_pages; p.pages = c.pages;
-    p.rows = t->B * c.heads * t->T;
     p.page_size = make_fast_divisor((uint32_t)c.page_size);
-    p.T = (int)t->T; p.H = (int)c.heads; p.d = (int)c.d;
+    p.T = (int)t->T; p.d = (int)c.d;
+    const int rows = rows_at_once(p.T, p.d);
+    p.blocks = make_fast_divisor((uint32_t)((p.T + rows - 1) / rows));
+    p.heads = make_fast_divisor((uint32_t)c.heads);
+    p.tasks = (int)(t->B * c.heads * p.blocks.divisor);
     p.status = ctx->d_status;
     const bool vec = (!t->k || vector_view(t->k, t->k_strides)) && (!t->v || vector_view(t->v, t->v_strides));
     cudaError_t e;

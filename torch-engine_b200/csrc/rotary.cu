@@ -27,82 +27,108 @@ struct RotaryParams {
     long long total;             // threads with work: tokens * head_lanes * items
     int T, H, rot, d;
     int head_lanes;              // threads that share the heads of a (token, item)
-    int rot_items, items;        // of a head: groups of pairs, then groups of copied elements
+    int rot_items, items;        // of a head: groups of W pairs, then of 2 W copied elements
     float scale, sign;
 };
 
-// W pairs (or W copied elements) a thread: W = 4 moves float4s and needs rot and d in multiples of 8 and 4, aligned views.
+// A thread takes two vectors of W elements of every head of a token: W pairs, or 2 W elements behind the rotated part (where they
+// are left as they are).  W = 4 moves float4s and needs rot in multiples of 8, d of 4, and aligned views.
+template <int W> struct Vector { float x[W]; };
+template <int W>
+__device__ __forceinline__ void load(Vector<W>& v, const float* p) {
+    if constexpr (W == 4) {
+        const float4 t = __ldcs(reinterpret_cast<const float4*>(p));
+        v.x[0] = t.x; v.x[1] = t.y; v.x[2] = t.z; v.x[3] = t.w;
+    } else {
+        v.x[0] = *p;
+    }
+}
+template <int W>
+__device__ __forceinline__ void store(float* p, const Vector<W>& v) {
+    if constexpr (W == 4) *reinterpret_cast<float4*>(p) = make_float4(v.x[0], v.x[1], v.x[2], v.x[3]);
+    else *p = v.x[0];
+}
+
 template <int W, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(256, 4) rotary_kernel(const RotaryParams p) {
     griddep_wait();
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= p.total) return;
-    long long rest = i / p.items;
-    const int item = (int)(i - rest * p.items);
-    const long long token = rest / p.head_lanes;
+    const unsigned rest = (unsigned)(i / p.items);          // (token, head lane): below 2^31
+    const int item = (int)(i - (long long)rest * p.items);
+    const unsigned token = rest / (unsigned)p.head_lanes;
     const int lane = (int)(rest - token * p.head_lanes);
-    const long long b = token / p.T;
+    const unsigned b = token / (unsigned)p.T;
     const int t = (int)(token - b * p.T);
+    const bool turned = item < p.rot_items;
+    const int j = item * W;                                  // first pair, where there are pairs
+    // element offsets of the thread's two vectors; interleaved pairs lie side by side in them
+    int o0 = INTERLEAVED ? 2 * j : j, o1 = INTERLEAVED ? 2 * j + W : j + p.rot / 2;
+    if (!turned) {
+        o0 = p.rot + (item - p.rot_items) * 2 * W;
+        o1 = o0 + W < p.d ? o0 + W : o0;                     // (the last vector may be alone: moved twice)
+    }
     const float* x = p.x + b * p.xs[0] + t * p.xs[2];
     float* y = p.y + b * p.ys[0] + t * p.ys[2];
-    if (item >= p.rot_items) {      // behind the rotated part
-        const int c = p.rot + (item - p.rot_items) * W;
-        for (int h = lane; h < p.H; h += p.head_lanes) {
-            if constexpr (W == 4) *reinterpret_cast<float4*>(y + h * p.ys[1] + c) = *reinterpret_cast<const float4*>(x + h * p.xs[1] + c);
-            else y[h * p.ys[1] + c] = x[h * p.xs[1] + c];
-        }
-        return;
-    }
-    const int j = item * W;         // first pair
-    const double position = (double)p.positions[b * p.ps[0] + t * p.ps[1]];
+    // two heads at a time, the next two under way; the first while the angles are computed
+    const int step = p.head_lanes;
+    Vector<W> u[2], v[2];
+    auto fetch = [&](int h) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (h + k * step < p.H) {
+                const float* xh = x + (h + k * step) * p.xs[1];
+                load(u[k], xh + o0);
+                load(v[k], xh + o1);
+            }
+    };
+    fetch(lane);
     float c[W], s[W];
+    if (turned) {
+        const double position = (double)p.positions[b * p.ps[0] + t * p.ps[1]];
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        const double turns = position * p.inv_freq[j + w] * 0.15915494309189535;      // 1 / (2 pi)
-        const float part = (float)(turns - rint(turns));
-        sincospif(2.0f * part, &s[w], &c[w]);
-        c[w] *= p.scale;
-        s[w] *= p.scale * p.sign;
+        for (int w = 0; w < W; ++w) {
+            const double turns = position * p.inv_freq[j + w] * 0.15915494309189535;      // 1 / (2 pi)
+            const float part = (float)(turns - rint(turns));
+            sincospif(2.0f * part, &s[w], &c[w]);
+            c[w] *= p.scale;
+            s[w] *= p.scale * p.sign;
+        }
     }
-    // element offsets of the thread's two vectors; interleaved pairs lie side by side in them
-    const int o0 = INTERLEAVED ? 2 * j : j, o1 = INTERLEAVED ? 2 * j + W : j + p.rot / 2;
-#pragma unroll 2
-    for (int h = lane; h < p.H; h += p.head_lanes) {
-        const float* xh = x + h * p.xs[1];
-        float* yh = y + h * p.ys[1];
-        float a[W], e[W];
-        if constexpr (W == 4) {
-            const float4 u = *reinterpret_cast<const float4*>(xh + o0), v = *reinterpret_cast<const float4*>(xh + o1);
-            a[0] = u.x; a[1] = u.y; a[2] = u.z; a[3] = u.w;
-            e[0] = v.x; e[1] = v.y; e[2] = v.z; e[3] = v.w;
-        } else {
-            a[0] = xh[o0];
-            e[0] = xh[o1];
-        }
-        if constexpr (INTERLEAVED && W == 4) {
+    for (int h = lane; h < p.H; h += 2 * step) {
+        Vector<W> a[2], e[2];
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const float u0 = a[2 * w], u1 = a[2 * w + 1], v0 = e[2 * w], v1 = e[2 * w + 1];
-                a[2 * w] = u0 * c[w] - u1 * s[w];
-                a[2 * w + 1] = u0 * s[w] + u1 * c[w];
-                e[2 * w] = v0 * c[w + 2] - v1 * s[w + 2];
-                e[2 * w + 1] = v0 * s[w + 2] + v1 * c[w + 2];
-            }
-        } else {
+        for (int k = 0; k < 2; ++k) { a[k] = u[k]; e[k] = v[k]; }
+        fetch(h + 2 * step);
+        if (turned) {
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float u = a[w], v = e[w];
-                a[w] = u * c[w] - v * s[w];
-                e[w] = u * s[w] + v * c[w];
+            for (int k = 0; k < 2; ++k) {
+                if constexpr (INTERLEAVED && W == 4) {
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const float a0 = a[k].x[2 * w], a1 = a[k].x[2 * w + 1], e0 = e[k].x[2 * w], e1 = e[k].x[2 * w + 1];
+                        a[k].x[2 * w] = a0 * c[w] - a1 * s[w];
+                        a[k].x[2 * w + 1] = a0 * s[w] + a1 * c[w];
+                        e[k].x[2 * w] = e0 * c[w + 2] - e1 * s[w + 2];
+                        e[k].x[2 * w + 1] = e0 * s[w + 2] + e1 * c[w + 2];
+                    }
+                } else {
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        const float a0 = a[k].x[w], e0 = e[k].x[w];
+                        a[k].x[w] = a0 * c[w] - e0 * s[w];
+                        e[k].x[w] = a0 * s[w] + e0 * c[w];
+                    }
+                }
             }
         }
-        if constexpr (W == 4) {
-            *reinterpret_cast<float4*>(yh + o0) = make_float4(a[0], a[1], a[2], a[3]);
-            *reinterpret_cast<float4*>(yh + o1) = make_float4(e[0], e[1], e[2], e[3]);
-        } else {
-            yh[o0] = a[0];
-            yh[o1] = e[0];
-        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (h + k * step < p.H) {
+                float* yh = y + (h + k * step) * p.ys[1];
+                store(yh + o0, a[k]);
+                store(yh + o1, e[k]);
+            }
     }
 }
 
@@ -174,12 +200,14 @@ int te_b200_rotary(te_b200_ctx* ctx, const te_rotary_desc* t, te_stream_t stream
     const bool vec = vector_view(t->x, t->x_strides) && vector_view(t->y, t->y_strides) && p.rot % 8 == 0 && p.d % 4 == 0;
     const int w = vec ? 4 : 1;
     p.rot_items = p.rot / (2 * w);
-    p.items = p.rot_items + (t->x == t->y ? 0 : (p.d - p.rot) / w);
+    p.items = p.rot_items + (t->x == t->y ? 0 : (p.d - p.rot + 2 * w - 1) / (2 * w));
     if (p.items == 0) return TE_OK;                  // in place with nothing to turn
-    // One thread per (token, item) when that fills the GPU; otherwise its heads are shared among several.
-    const long long base = t->B * t->T * p.items, fill = (long long)ctx->sm_count * 2048;
-    long long lanes = (fill + base - 1) / base;
-    p.head_lanes = (int)(lanes > p.H ? p.H : lanes);
+    // One thread per (token, item) where that fills the GPU (four blocks of 256 threads per SM); otherwise its heads are shared
+    // among several.
+    const long long tokens = t->B * t->T, base = tokens * p.items, fill = (long long)ctx->sm_count * 1024;
+    long long lanes = fill / base;
+    lanes = lanes < 1 ? 1 : lanes > p.H ? p.H : lanes;
+    p.head_lanes = (int)lanes;
     p.total = base * p.head_lanes;
     const long long blocks = (p.total + 255) / 256;
     if (blocks > INT32_MAX) return fail(TE_ERR_BAD_ARGUMENT, "rotary: too many elements");
