@@ -6,7 +6,8 @@
 // for d > 128), so that FP32 moves in float4s, the largest magnitude of a row is one reduction within the group, and a
 // row's bytes leave in one coalesced store.  A group moves ROWS consecutive tokens of one head (of k and of v) at once: they lie
 // side by side in the cache's usual order [pages, heads, page_size, d], and their positions, page numbers and data are
-// three loads one after the other that ROWS tokens wait for together.
+// three loads one after the other that ROWS tokens wait for together.  Each lane works out the place of one of these
+// tokens and the others take it from there.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -65,7 +66,7 @@ __device__ __forceinline__ void store4(float* p, float4 x) {
 
 // Values of one row into the cache at `row`; `x` is this lane's part, element 4 * (lane + LANES * u) + i in x[u] component i.
 template <int DTYPE, int LANES, int U>
-__device__ __forceinline__ void put_row(const float4 (&x)[U], typename Stored<DTYPE>::type* row, float* scale, int lane, int d, bool there, unsigned mask) {
+__device__ __forceinline__ void put_row(const float4 (&x)[U], typename Stored<DTYPE>::type* row, float* scale, bool write_scale, int lane, int d, bool there, unsigned mask) {
     float inv = 1.0f;
     bool finite = true;
     if constexpr (DTYPE == TE_KV_E4M3) {
@@ -88,7 +89,7 @@ __device__ __forceinline__ void put_row(const float4 (&x)[U], typename Stored<DT
         }
         const int e = scale_exponent(__uint_as_float(top));
         inv = power_of_two(-e);
-        if (there && lane == 0) *scale = power_of_two(e);
+        if (write_scale) *scale = power_of_two(e);
     }
     if (!there) return;
 #pragma unroll
@@ -117,15 +118,17 @@ __device__ __forceinline__ void put_row(const float4 (&x)[U], typename Stored<DT
     }
 }
 
+// Four elements as they are stored, and as FP32.
+template <int DTYPE> struct Raw { typedef float4 type; };
+template <> struct Raw<TE_KV_BF16> { typedef uint2 type; };
+template <> struct Raw<TE_KV_E4M3> { typedef unsigned type; };
 template <int DTYPE>
-__device__ __forceinline__ float4 get4(const typename Stored<DTYPE>::type* p, float scale) {
+__device__ __forceinline__ float4 values_of(const typename Raw<DTYPE>::type& w, float scale) {
     if constexpr (DTYPE == TE_KV_F32) {
-        return *reinterpret_cast<const float4*>(p);
+        return w;
     } else if constexpr (DTYPE == TE_KV_BF16) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
         return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
     } else {
-        const unsigned w = *reinterpret_cast<const unsigned*>(p);
         const float2 lo = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3)));
         const float2 hi = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3)));
         return make_float4(lo.x * scale, lo.y * scale, hi.x * scale, hi.y * scale);
@@ -136,101 +139,108 @@ template <int DTYPE, int LANES, int U, int ROWS, bool VEC, bool APPEND>
 __global__ void __launch_bounds__(256) kv_move_kernel(const KvParams p) {
     griddep_wait();
     typedef typename Stored<DTYPE>::type S;
+    typedef typename Raw<DTYPE>::type W;
     constexpr int GROUPS = 256 / LANES;
+    static_assert(ROWS <= LANES, "a lane per token");
     const int lane = threadIdx.x % LANES;
     const unsigned task = blockIdx.x * GROUPS + threadIdx.x / LANES;
-    const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << (threadIdx.x % 32 / LANES * LANES);
+    const int first_lane = threadIdx.x % 32 / LANES * LANES;
+    const unsigned mask = LANES == 32 ? 0xffffffffu : ((1u << LANES) - 1u) << first_lane;
     if (task >= (unsigned)p.tasks) return;            // the whole group leaves
     const unsigned bh = fast_quotient(task, p.blocks);
     const int t0 = (int)(task - bh * p.blocks.divisor) * ROWS;
     const unsigned b = fast_quotient(bh, p.heads);
     const int h = (int)(bh - b * p.heads.divisor);
     const int64_t* positions = p.positions + b * p.ps[0];
-    const PageRow table = {p.page_table + b * p.table_stride, p.max_pages, p.pages};
-    float* k = p.k + b * p.ks[0] + h * p.ks[1];
-    float* v = p.v + b * p.vs[0] + h * p.vs[1];
-    int64_t position[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) position[i] = t0 + i < p.T ? positions[(t0 + i) * p.ps[1]] : -1;
+    const int own = lane % ROWS;                       // the token whose place this lane works out
+    const int64_t position = t0 + own < p.T ? positions[(t0 + own) * p.ps[1]] : -1;
+    const unsigned wanted = __ballot_sync(mask, position >= 0) >> first_lane;        // not padding: bit i for token i
+    if (APPEND && (wanted & ((1u << ROWS) - 1u)) == 0u) return;
     const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    float4 x[ROWS][U], y[ROWS][U];
+    float4 x[APPEND ? ROWS : 1][U], y[APPEND ? ROWS : 1][U];
+    float* k = p.k + b * p.ks[0] + h * p.ks[1] + t0 * p.ks[2] + 4 * lane;
+    float* v = p.v + b * p.vs[0] + h * p.vs[1] + t0 * p.vs[2] + 4 * lane;
     if constexpr (APPEND) {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int c = 4 * (lane + LANES * u);
-                const bool in = position[i] >= 0 && c < p.d;       // (nothing is read of padding)
-                x[i][u] = in ? load4<VEC>(k + (t0 + i) * p.ks[2] + c) : zero;
-                y[i][u] = in ? load4<VEC>(v + (t0 + i) * p.vs[2] + c) : zero;
+                const bool in = (wanted >> i & 1u) && 4 * (lane + LANES * u) < p.d;       // (nothing is read of padding)
+                x[i][u] = in ? load4<VEC>(k + i * p.ks[2] + 4 * LANES * u) : zero;
+                y[i][u] = in ? load4<VEC>(v + i * p.vs[2] + 4 * LANES * u) : zero;
             }
     }
-    int64_t page[ROWS];
-    uint32_t slot[ROWS];
-    bool there[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        page[i] = 0;
-        slot[i] = 0u;
-        there[i] = kv_place(table, p.page_size, position[i], page[i], slot[i]);
-        if (!there[i]) {
-            if (position[i] >= 0 && lane == 0) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
-            page[i] = 0;
-        }
-    }
+    const PageRow table = {p.page_table + b * p.table_stride, p.max_pages, p.pages};
+    int64_t page = 0;
+    uint32_t slot = 0;
+    const bool found = kv_place(table, p.page_size, position, page, slot);
+    if (!found && position >= 0 && lane < ROWS) atomicCAS(p.status, 0, STATUS_BAD_CACHE_PLACE);
+    const unsigned there = __ballot_sync(mask, found) >> first_lane;
+    const unsigned at = found ? (unsigned)page : 0u;   // (pages of a cache are below 2^31)
+    if (!found) slot = 0u;
+    const long long ka = at * p.kcs[0] + slot * p.kcs[2], va = at * p.vcs[0] + slot * p.vcs[2];
+    S* kc = static_cast<S*>(p.kc) + h * p.kcs[1];
+    S* vc = static_cast<S*>(p.vc) + h * p.vcs[1];
+    const int64_t sa = DTYPE == TE_KV_E4M3 ? at * p.ss[0] + h * p.ss[1] + slot * p.ss[2] : 0;
     if constexpr (APPEND) {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            const int64_t s = DTYPE == TE_KV_E4M3 ? page[i] * p.ss[0] + h * p.ss[1] + slot[i] * p.ss[2] : 0;
-            put_row<DTYPE, LANES, U>(x[i], static_cast<S*>(p.kc) + page[i] * p.kcs[0] + h * p.kcs[1] + slot[i] * p.kcs[2], p.k_scale + s, lane, p.d, there[i], mask);
-            put_row<DTYPE, LANES, U>(y[i], static_cast<S*>(p.vc) + page[i] * p.vcs[0] + h * p.vcs[1] + slot[i] * p.vcs[2], p.v_scale + s, lane, p.d, there[i], mask);
+            const bool to = there >> i & 1u;
+            const long long kr = __shfl_sync(mask, ka, first_lane + i), vr = __shfl_sync(mask, va, first_lane + i);
+            put_row<DTYPE, LANES, U>(x[i], kc + kr, p.k_scale + sa, to && lane == i, lane, p.d, to, mask);
+            put_row<DTYPE, LANES, U>(y[i], vc + vr, p.v_scale + sa, to && lane == i, lane, p.d, to, mask);
         }
     } else {
+        W kw[ROWS][U] = {}, vw[ROWS][U] = {};
+        float ks = 1.0f, vs = 1.0f;
+        if (DTYPE == TE_KV_E4M3 && found) {
+            if (p.k) ks = p.k_scale[sa];
+            if (p.v) vs = p.v_scale[sa];
+        }
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            float sk = 1.0f, sv = 1.0f;
-            if (DTYPE == TE_KV_E4M3 && there[i]) {
-                const int64_t s = page[i] * p.ss[0] + h * p.ss[1] + slot[i] * p.ss[2];
-                if (p.k) sk = p.k_scale[s];
-                if (p.v) sv = p.v_scale[s];
-            }
-            const S* kr = static_cast<const S*>(p.kc) + page[i] * p.kcs[0] + h * p.kcs[1] + slot[i] * p.kcs[2];
-            const S* vr = static_cast<const S*>(p.vc) + page[i] * p.vcs[0] + h * p.vcs[1] + slot[i] * p.vcs[2];
+            const long long kr = __shfl_sync(mask, ka, first_lane + i), vr = __shfl_sync(mask, va, first_lane + i);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int c = 4 * (lane + LANES * u);
-                const bool in = there[i] && c < p.d;
-                x[i][u] = in && p.k ? get4<DTYPE>(kr + c, sk) : zero;
-                y[i][u] = in && p.v ? get4<DTYPE>(vr + c, sv) : zero;
+                const bool in = (there >> i & 1u) && c < p.d;
+                if (in && p.k) kw[i][u] = *reinterpret_cast<const W*>(kc + kr + c);
+                if (in && p.v) vw[i][u] = *reinterpret_cast<const W*>(vc + vr + c);
             }
         }
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
-            if (t0 + i >= p.T) break;
+            const float sk = DTYPE == TE_KV_E4M3 ? __shfl_sync(mask, ks, first_lane + i) : 1.0f;
+            const float sv = DTYPE == TE_KV_E4M3 ? __shfl_sync(mask, vs, first_lane + i) : 1.0f;
+            if (t0 + i >= p.T) continue;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int c = 4 * (lane + LANES * u);
-                if (c >= p.d) continue;
-                if (p.k) store4<VEC>(k + (t0 + i) * p.ks[2] + c, x[i][u]);
-                if (p.v) store4<VEC>(v + (t0 + i) * p.vs[2] + c, y[i][u]);
+                if (4 * (lane + LANES * u) >= p.d) continue;
+                if (p.k) store4<VEC>(k + i * p.ks[2] + 4 * LANES * u, values_of<DTYPE>(kw[i][u], sk));
+                if (p.v) store4<VEC>(v + i * p.vs[2] + 4 * LANES * u, values_of<DTYPE>(vw[i][u], sv));
             }
         }
     }
 }
 
-// Tokens a group moves at once: four (two of the longest rows), one where there are few per sequence.
-int rows_at_once(int T, int d) { return T < 4 ? 1 : d > 128 ? 2 : 4; }
+// Tokens a group moves at once: one where there are few per sequence, else so many that about 1 KB of a lane group's loads is
+// under way.
+int rows_at_once(int dtype, int T, int d, bool append) {
+    if (T < 4) return 1;
+    return !append && dtype != TE_KV_F32 && d <= 128 ? 8 : d > 128 ? 2 : 4;
+}
 
 template <int DTYPE, bool APPEND>
 cudaError_t launch_move(const KvParams& p, bool vec, cudaStream_t st) {
-    const int lanes = p.d <= 32 ? 8 : p.d <= 64 ? 16 : 32, rows = rows_at_once(p.T, p.d);
+    constexpr int MANY = !APPEND && DTYPE != TE_KV_F32 ? 8 : 4;
+    const int lanes = p.d <= 32 ? 8 : p.d <= 64 ? 16 : 32, rows = rows_at_once(DTYPE, p.T, p.d, APPEND);
     const int groups = 256 / lanes;
-    const dim3 grid((unsigned)((p.tasks + groups - 1) / groups)), block(256);
+    const dim3 grid((unsigned)(((unsigned)p.tasks + groups - 1) / groups)), block(256);
 #define TE_MOVE(L, U, N) (vec ? launch_pdl(kv_move_kernel<DTYPE, L, U, N, true, APPEND>, grid, block, 0, st, p) \
                               : launch_pdl(kv_move_kernel<DTYPE, L, U, N, false, APPEND>, grid, block, 0, st, p))
-    if (lanes == 8) return rows == 1 ? TE_MOVE(8, 1, 1) : TE_MOVE(8, 1, 4);
-    if (lanes == 16) return rows == 1 ? TE_MOVE(16, 1, 1) : TE_MOVE(16, 1, 4);
-    if (p.d <= 128) return rows == 1 ? TE_MOVE(32, 1, 1) : TE_MOVE(32, 1, 4);
+    if (lanes == 8) return rows == 1 ? TE_MOVE(8, 1, 1) : TE_MOVE(8, 1, MANY);
+    if (lanes == 16) return rows == 1 ? TE_MOVE(16, 1, 1) : TE_MOVE(16, 1, MANY);
+    if (p.d <= 128) return rows == 1 ? TE_MOVE(32, 1, 1) : TE_MOVE(32, 1, MANY);
     return rows == 1 ? TE_MOVE(32, 2, 1) : TE_MOVE(32, 2, 2);
 #undef TE_MOVE
 }
@@ -273,7 +283,7 @@ int move(te_b200_ctx* ctx, const te_kv_desc* t, bool append, cudaStream_t st) {
     p.table_stride = t->page_table_stride; p.max_pages = t->max_pages; p.pages = c.pages;
     p.page_size = make_fast_divisor((uint32_t)c.page_size);
     p.T = (int)t->T; p.d = (int)c.d;
-    const int rows = rows_at_once(p.T, p.d);
+    const int rows = rows_at_once(c.dtype, p.T, p.d, append);
     p.blocks = make_fast_divisor((uint32_t)((p.T + rows - 1) / rows));
     p.heads = make_fast_divisor((uint32_t)c.heads);
     p.tasks = (int)(t->B * c.heads * p.blocks.divisor);
@@ -294,6 +304,7 @@ int check_kv_cache(const te_kv_cache& c, const char* who) {
     const std::string name = who;
     if (c.dtype < TE_KV_F32 || c.dtype > TE_KV_E4M3) return fail(TE_ERR_BAD_ARGUMENT, name + ": cache dtype must be a TE_KV_* value");
     if (c.pages < 0 || c.heads < 0) return fail(TE_ERR_BAD_ARGUMENT, name + ": bad cache extents");
+    if (c.pages > INT32_MAX) return fail(TE_ERR_BAD_ARGUMENT, name + ": more than 2^31-1 pages");
     if (c.heads > 65535) return fail(TE_ERR_BAD_ARGUMENT, name + ": more than 65535 cache heads");
     if (c.page_size < 1 || c.page_size > INT32_MAX) return fail(TE_ERR_BAD_ARGUMENT, name + ": page_size must be between 1 and 2^31-1");
     if (c.d < 16 || c.d > 256 || c.d % 16) return fail(TE_ERR_BAD_ARGUMENT, name + ": d must be a multiple of 16 between 16 and 256");

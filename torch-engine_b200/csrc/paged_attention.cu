@@ -1131,7 +1131,6 @@ int check_desc(const te_paged_attn_desc* t) {
     const te_kv_cache& c = t->cache;
     if (t->q_heads > 0 && (c.heads == 0 || t->q_heads % c.heads)) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: q_heads must be a multiple of the cache's heads");
     if (t->max_pages > 0 && c.page_size > (INT32_MAX - 4096) / t->max_pages) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: the page table reaches beyond 2^31-1 positions");
-    if (c.pages > INT32_MAX) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: more than 2^31-1 pages");
     if (t->q_heads > 65535 || (t->q_heads > 0 && t->rows > INT32_MAX / t->q_heads)) return fail(TE_ERR_BAD_ARGUMENT, "paged attention: too many rows or heads");
     if (t->max_pages > 0 && (t->max_pages * c.page_size / 32 + 4) * t->q_heads >= INT32_MAX)
         return fail(TE_ERR_BAD_ARGUMENT, "paged attention: too many heads for so long a page table");

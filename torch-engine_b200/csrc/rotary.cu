@@ -61,21 +61,25 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const RotaryParams p) {
     const unsigned b = token / (unsigned)p.T;
     const int t = (int)(token - b * p.T);
     const bool turned = item < p.rot_items;
-    const int j = item * W;                                  // first pair, where there are pairs
-    // element offsets of the thread's two vectors; interleaved pairs lie side by side in them
-    int o0 = INTERLEAVED ? 2 * j : j, o1 = INTERLEAVED ? 2 * j + W : j + p.rot / 2;
+    // Element offsets of the thread's two vectors, half the rotated (or the copied) part apart, so that a warp's accesses are
+    // contiguous in either layout; and the pairs their elements belong to: W from j0, or (interleaved) W / 2 from j0 and from j1.
+    int o0 = item * W, o1 = o0 + p.rot / 2;
+    const int j0 = INTERLEAVED && W == 4 ? o0 / 2 : o0, j1 = INTERLEAVED && W == 4 ? o1 / 2 : 0;
+    if (INTERLEAVED && W == 1) { o0 = 2 * item; o1 = o0 + 1; }
     if (!turned) {
-        o0 = p.rot + (item - p.rot_items) * 2 * W;
-        o1 = o0 + W < p.d ? o0 + W : o0;                     // (the last vector may be alone: moved twice)
+        const int vectors = (p.d - p.rot) / W, half = (vectors + 1) / 2, k = item - p.rot_items;
+        o0 = p.rot + k * W;
+        o1 = k + half < vectors ? o0 + half * W : o0;        // (the last vector may be alone: moved twice)
     }
     const float* x = p.x + b * p.xs[0] + t * p.xs[2];
     float* y = p.y + b * p.ys[0] + t * p.ys[2];
-    // two heads at a time, the next two under way; the first while the angles are computed
+    // several heads at a time; the first are under way while the angles are computed
+    constexpr int N = 4;
     const int step = p.head_lanes;
-    Vector<W> u[2], v[2];
+    Vector<W> u[N], v[N];
     auto fetch = [&](int h) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < N; ++k)
             if (h + k * step < p.H) {
                 const float* xh = x + (h + k * step) * p.xs[1];
                 load(u[k], xh + o0);
@@ -88,46 +92,44 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const RotaryParams p) {
         const double position = (double)p.positions[b * p.ps[0] + t * p.ps[1]];
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const double turns = position * p.inv_freq[j + w] * 0.15915494309189535;      // 1 / (2 pi)
+            const int j = INTERLEAVED && W == 4 && w >= 2 ? j1 + w - 2 : j0 + w;
+            const double turns = position * p.inv_freq[j] * 0.15915494309189535;      // 1 / (2 pi)
             const float part = (float)(turns - rint(turns));
             sincospif(2.0f * part, &s[w], &c[w]);
             c[w] *= p.scale;
             s[w] *= p.scale * p.sign;
         }
     }
-    for (int h = lane; h < p.H; h += 2 * step) {
-        Vector<W> a[2], e[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) { a[k] = u[k]; e[k] = v[k]; }
-        fetch(h + 2 * step);
+    for (int h = lane; h < p.H; h += N * step) {
+        if (h != lane) fetch(h);
         if (turned) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < N; ++k) {
                 if constexpr (INTERLEAVED && W == 4) {
 #pragma unroll
                     for (int w = 0; w < 2; ++w) {
-                        const float a0 = a[k].x[2 * w], a1 = a[k].x[2 * w + 1], e0 = e[k].x[2 * w], e1 = e[k].x[2 * w + 1];
-                        a[k].x[2 * w] = a0 * c[w] - a1 * s[w];
-                        a[k].x[2 * w + 1] = a0 * s[w] + a1 * c[w];
-                        e[k].x[2 * w] = e0 * c[w + 2] - e1 * s[w + 2];
-                        e[k].x[2 * w + 1] = e0 * s[w + 2] + e1 * c[w + 2];
+                        const float a0 = u[k].x[2 * w], a1 = u[k].x[2 * w + 1], e0 = v[k].x[2 * w], e1 = v[k].x[2 * w + 1];
+                        u[k].x[2 * w] = a0 * c[w] - a1 * s[w];
+                        u[k].x[2 * w + 1] = a0 * s[w] + a1 * c[w];
+                        v[k].x[2 * w] = e0 * c[w + 2] - e1 * s[w + 2];
+                        v[k].x[2 * w + 1] = e0 * s[w + 2] + e1 * c[w + 2];
                     }
                 } else {
 #pragma unroll
                     for (int w = 0; w < W; ++w) {
-                        const float a0 = a[k].x[w], e0 = e[k].x[w];
-                        a[k].x[w] = a0 * c[w] - e0 * s[w];
-                        e[k].x[w] = a0 * s[w] + e0 * c[w];
+                        const float a0 = u[k].x[w], e0 = v[k].x[w];
+                        u[k].x[w] = a0 * c[w] - e0 * s[w];
+                        v[k].x[w] = a0 * s[w] + e0 * c[w];
                     }
                 }
             }
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int k = 0; k < N; ++k)
             if (h + k * step < p.H) {
                 float* yh = y + (h + k * step) * p.ys[1];
-                store(yh + o0, a[k]);
-                store(yh + o1, e[k]);
+                store(yh + o0, u[k]);
+                store(yh + o1, v[k]);
             }
     }
 }
