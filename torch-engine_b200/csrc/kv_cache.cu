@@ -223,16 +223,17 @@ __global__ void __launch_bounds__(256) kv_move_kernel(const KvParams p) {
     }
 }
 
-// Tokens a group moves at once: one where there are few per sequence, else so many that about 1 KB of a lane group's loads is
-// under way.
+// Tokens a group moves at once: one where there are few per sequence; else two rows of FP32 in and out, or up to four (written)
+// or eight (read) of the narrower types.
+constexpr int MOST_F32 = 2, MOST_APPENDED = 4, MOST_READ = 8;
 int rows_at_once(int dtype, int T, int d, bool append) {
     if (T < 4) return 1;
-    return !append && dtype != TE_KV_F32 && d <= 128 ? 8 : d > 128 ? 2 : 4;
+    return dtype == TE_KV_F32 || d > 128 ? MOST_F32 : append ? MOST_APPENDED : MOST_READ;
 }
 
 template <int DTYPE, bool APPEND>
 cudaError_t launch_move(const KvParams& p, bool vec, cudaStream_t st) {
-    constexpr int MANY = !APPEND && DTYPE != TE_KV_F32 ? 8 : 4;
+    constexpr int MANY = DTYPE == TE_KV_F32 ? MOST_F32 : APPEND ? MOST_APPENDED : MOST_READ;
     const int lanes = p.d <= 32 ? 8 : p.d <= 64 ? 16 : 32, rows = rows_at_once(DTYPE, p.T, p.d, APPEND);
     const int groups = 256 / lanes;
     const dim3 grid((unsigned)(((unsigned)p.tasks + groups - 1) / groups)), block(256);
@@ -241,7 +242,7 @@ cudaError_t launch_move(const KvParams& p, bool vec, cudaStream_t st) {
     if (lanes == 8) return rows == 1 ? TE_MOVE(8, 1, 1) : TE_MOVE(8, 1, MANY);
     if (lanes == 16) return rows == 1 ? TE_MOVE(16, 1, 1) : TE_MOVE(16, 1, MANY);
     if (p.d <= 128) return rows == 1 ? TE_MOVE(32, 1, 1) : TE_MOVE(32, 1, MANY);
-    return rows == 1 ? TE_MOVE(32, 2, 1) : TE_MOVE(32, 2, 2);
+    return rows == 1 ? TE_MOVE(32, 2, 1) : TE_MOVE(32, 2, MOST_F32);
 #undef TE_MOVE
 }
 

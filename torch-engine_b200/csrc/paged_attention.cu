@@ -38,8 +38,11 @@ constexpr int THREADS = 32 * WARPS;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
-// Thread blocks per SM
-constexpr int blocks_per_sm(int dtype, int d) { return dtype == TE_KV_E4M3 ? (d <= 128 ? 3 : 2) : d <= 128 ? (dtype == TE_KV_BF16 ? 3 : 2) : 1; }
+// Thread blocks per SM, a power of the registers and the rings: three with two stages each where 168 registers a thread will do
+// and two stages of a block's four warps take at most 66 KB, else two with three stages, one for the longest rows.
+constexpr int blocks_per_sm(int dtype, int d, int heads) {
+    return dtype == TE_KV_E4M3 ? (d <= 128 ? 3 : 2) : d > 128 ? 1 : dtype == TE_KV_BF16 || heads <= 2 ? 3 : 2;
+}
 
 struct AttnParams {
     const float* q;
@@ -322,7 +325,7 @@ struct TensorWarp {
     static constexpr int ES = E4M3 ? 1 : 2;
     static constexpr int TOKENS = DP * ES <= 128 ? 32 : 16;             // 8 KB a stage (16 for bf16 rows of 256)
     static constexpr int NK = TOKENS / 16;
-    static constexpr int BLOCKS = blocks_per_sm(DTYPE, DP);
+    static constexpr int BLOCKS = blocks_per_sm(DTYPE, DP, HT);
     typedef Ring<DP, ES, TOKENS, BLOCKS == 3 ? 2 : 3, E4M3, PACKED> R;
     static constexpr int KG = E4M3 ? DP / 64 : DP / 32;                 // groups of 4 lanes x 16 bytes of a key
     static constexpr int VW = E4M3 && DP < 128 ? 8 : 16;                // bytes of a value a lane holds per chunk
@@ -619,7 +622,7 @@ template <int DP, int HT, bool PACKED>
 struct FmaWarp {
     static constexpr int HEADS = HT;
     static constexpr int TOKENS = DP <= 64 ? 16 : 8;
-    static constexpr int BLOCKS = blocks_per_sm(TE_KV_F32, DP);
+    static constexpr int BLOCKS = blocks_per_sm(TE_KV_F32, DP, HT);
     typedef Ring<DP, 4, TOKENS, BLOCKS == 3 ? 2 : 3, false, PACKED> R;
     static constexpr int TG = TOKENS / 8;                  // tokens whose keys a lane takes parts of
     static constexpr int KC = DP / 16;                     // 16-byte pieces of a key a lane takes
@@ -1089,7 +1092,8 @@ int heads_per_tile(int dtype, int64_t group) {
 
 size_t workspace_need(const te_paged_attn_desc* t, int sm_count) {
     if (t->rows == 0 || t->q_heads == 0) return 0;
-    const size_t workers = (size_t)sm_count * blocks_per_sm(t->cache.dtype, (int)t->cache.d), heads = heads_per_tile(t->cache.dtype, t->q_heads / t->cache.heads);
+    const int tile = heads_per_tile(t->cache.dtype, t->q_heads / t->cache.heads);
+    const size_t workers = (size_t)sm_count * blocks_per_sm(t->cache.dtype, (int)t->cache.d, tile), heads = tile;
     return workers * 16 + 2 * workers * heads * (8 + 4 * (size_t)t->cache.d);
 }
 
@@ -1171,7 +1175,6 @@ int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* t, te_st
         snprintf(msg, sizeof msg, "context workspace (%zu bytes) too small; paged attention needs %zu bytes", ctx->workspace_bytes, need);
         return fail(TE_ERR_WORKSPACE, msg);
     }
-    const int workers = ctx->sm_count * blocks_per_sm(c.dtype, (int)c.d);
     AttnParams p;
     p.kc = static_cast<const char*>(c.k); p.vc = static_cast<const char*>(c.v); p.k_scale = c.k_scale; p.v_scale = c.v_scale;
     const int64_t size = c.dtype == TE_KV_F32 ? 4 : c.dtype == TE_KV_BF16 ? 2 : 1;
@@ -1183,6 +1186,7 @@ int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* t, te_st
     p.q_heads = (int)t->q_heads; p.kv_heads = (int)c.heads;
     p.group = (int)(t->q_heads / c.heads); p.d = (int)c.d;
     const int heads = heads_per_tile(c.dtype, p.group);
+    const int workers = ctx->sm_count * blocks_per_sm(c.dtype, p.d, heads);
     p.head_tiles = (p.group + heads - 1) / heads;
     p.scale = t->scale;
     char* ws = static_cast<char*>(ctx->workspace);
