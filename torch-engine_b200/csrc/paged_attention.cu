@@ -152,6 +152,11 @@ __device__ __forceinline__ float2 unpair(unsigned long long v) {
 __device__ __forceinline__ void fma2(unsigned long long& d, unsigned long long a, unsigned long long b) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(d) : "l"(a), "l"(b));
 }
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
     unsigned long long d;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
@@ -228,9 +233,13 @@ struct Ring {
         const char* kc = p.kc + kv_head * p.kcs[1];
         const char* vc = p.vc + kv_head * p.vcs[1];
         // tokens inside the range, then those on pages of the cache
+        constexpr unsigned ALL = 0xffffffffu >> (32 - TOKENS);
         const int lo = range.first - t0, hi = range.n - t0;
-        unsigned seen = hi <= 0 ? 0u : hi >= TOKENS ? 0xffffffffu >> (32 - TOKENS) : (1u << hi) - 1u;
-        if (lo > 0) seen = lo >= TOKENS ? 0u : seen & ~((1u << lo) - 1u);
+        unsigned seen = ALL;
+        if (lo > 0 || hi < TOKENS) {
+            seen = hi <= 0 ? 0u : hi >= TOKENS ? ALL : (1u << hi) - 1u;
+            if (lo > 0) seen = lo >= TOKENS ? 0u : seen & ~((1u << lo) - 1u);
+        }
         unsigned good = 0u;
         if constexpr (PACKED) {
 #pragma unroll
@@ -248,8 +257,8 @@ struct Ring {
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const bool there = (good >> (b * BLOCK)) & 1u;
-                k[b] = kc + (there ? entry[b] * p.kcs[0] + slot[b] * (int64_t)RB : 0) + lane * 16;
-                v[b] = vc + (there ? entry[b] * p.vcs[0] + slot[b] * (int64_t)RB : 0) + lane * 16;
+                k[b] = kc + (there ? (unsigned)entry[b] * p.kcs[0] + (unsigned long long)slot[b] * RB : 0) + lane * 16;
+                v[b] = vc + (there ? (unsigned)entry[b] * p.vcs[0] + (unsigned long long)slot[b] * RB : 0) + lane * 16;
             }
             auto copy = [&](auto whole) {
 #pragma unroll
@@ -268,32 +277,38 @@ struct Ring {
                     }
                 }
             };
-            if (seen == 0xffffffffu >> (32 - TOKENS)) copy(std::true_type());
+            if (seen == ALL) copy(std::true_type());
             else copy(std::false_type());
         } else {
-            const int page = good >> lane & 1u ? (int)entry[0] : 0;
+            const unsigned page = good >> lane & 1u ? (unsigned)entry[0] : 0u;
+            const long long ko = page * p.kcs[0] + slot[0] * p.kcs[2], vo = page * p.vcs[0] + slot[0] * p.vcs[2];
+            const bool same = p.kcs[0] == p.vcs[0] && p.kcs[2] == p.vcs[2];
+            const int width = p.d * ES;
+            auto copy = [&](auto same_places) {
 #pragma unroll
-            for (int c = 0; c < TOKENS / TPI; ++c) {
-                const int t = c * TPI + sub;
-                const int64_t at = __shfl_sync(0xffffffffu, page, t);
-                const int64_t in = __shfl_sync(0xffffffffu, slot[0], t);
-                const char* k = kc + at * p.kcs[0] + in * p.kcs[2];
-                const char* v = vc + at * p.vcs[0] + in * p.vcs[2];
+                for (int c = 0; c < TOKENS / TPI; ++c) {
+                    const int t = c * TPI + sub;
+                    const long long k = __shfl_sync(0xffffffffu, ko, t);
+                    const long long v = decltype(same_places)::value ? k : __shfl_sync(0xffffffffu, vo, t);
 #pragma unroll
-                for (int u = 0; u < PPR; ++u) {
-                    const int j = chunk + 32 * u;
-                    const bool there = (seen >> t & 1u) && j * 16 < p.d * ES;
-                    copy16_or_zero(to + key_at(t, j), k + (there ? j * 16 : 0), there);
-                    copy16_or_zero(to + SIDE + value_at(t, j), v + (there ? j * 16 : 0), there);
+                    for (int u = 0; u < PPR; ++u) {
+                        const int j = chunk + 32 * u;
+                        const bool there = (seen >> t & 1u) && j * 16 < width;
+                        const int byte = there ? j * 16 : 0;
+                        copy16_or_zero(to + key_at(t, j), kc + k + byte, there);
+                        copy16_or_zero(to + SIDE + value_at(t, j), vc + v + byte, there);
+                    }
                 }
-            }
+            };
+            if (same) copy(std::true_type());
+            else copy(std::false_type());
         }
         if constexpr (SCALES) {          // lane t copies token t's
             int64_t at = 0;
             const bool mine = lane < TOKENS && (seen >> (lane % TOKENS) & 1u);
             if constexpr (PACKED) {
                 const bool second = NB > 1 && lane >= BLOCK;
-                at = (second ? entry[NB - 1] : entry[0]) * p.ss[0] + (int64_t)((second ? slot[NB - 1] : slot[0]) + lane % BLOCK) * p.ss[2];
+                at = (second ? (unsigned)entry[NB - 1] : (unsigned)entry[0]) * p.ss[0] + ((second ? slot[NB - 1] : slot[0]) + lane % BLOCK) * p.ss[2];
             } else {
                 at = entry[0] * p.ss[0] + (int64_t)slot[0] * p.ss[2];
             }
@@ -408,24 +423,27 @@ struct TensorWarp {
         }
     }
 
-    float acc[VC * VE][2];     // [n tile][2 columns] of head g, both rows of its terms
+    unsigned long long acc[VC * VE];     // [n tile]: 2 columns of head g, both rows of its terms
     float m, l;                // of head g; l over this lane's tokens only
     float mv;                  // e4m3: the maximum the values' weights are measured against
     float unit;                // what a score is multiplied by
+    int width;                 // d: !PACKED products behind it are left out
 
     // The tensor core truncates as it adds to its accumulator, which over many tokens would shrink the sums; so each 16 tokens'
     // product starts from zero and is added here, rounded to nearest, with the rescaling in the same FMA.
-    __device__ __forceinline__ void add(int i, const float (&x)[4], float keep) {
-        acc[i][0] = fmaf(acc[i][0], keep, x[0] + x[2]);
-        acc[i][1] = fmaf(acc[i][1], keep, x[1] + x[3]);
+    __device__ __forceinline__ void add(int i, const float (&x)[4], unsigned long long keep) {
+        unsigned long long sum = add2(pair(x[0], x[1]), pair(x[2], x[3]));
+        fma2(sum, acc[i], keep);
+        acc[i] = sum;
     }
 
     __device__ __forceinline__ void begin(const AttnParams& p, const float* q_unit) {
 #pragma unroll
-        for (int i = 0; i < VC * VE; ++i) acc[i][0] = acc[i][1] = 0.0f;
+        for (int i = 0; i < VC * VE; ++i) acc[i] = 0ull;
         m = mv = -INFINITY;
         l = 0.0f;
         unit = p.scale * LOG2E * (E4M3 ? q_unit[threadIdx.x % 32 / 4] : 1.0f);
+        width = p.d;
     }
 
     // One stage's tokens, those of the bits of `seen`.
@@ -439,6 +457,7 @@ struct TensorWarp {
             float sc[2 * NK][2][4];
 #pragma unroll
             for (int c = 0; c < KG; ++c) {
+                if (!PACKED && c > 0 && c * (4 * 16 / ES) >= width) break;
                 const uint4* q = reinterpret_cast<const uint4*>(words) + c * KQ * 32 + lane;
                 uint4 qw[KQ];
 #pragma unroll
@@ -466,22 +485,35 @@ struct TensorWarp {
             float w[NK][4], vs[NK][4];
             float top = -INFINITY, topv = -INFINITY;
 #pragma unroll
-            for (int nk = 0; nk < NK; ++nk)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = nk * 16 + 8 * (i / 2) + 2 * r + i % 2;
-                    const float (&y)[4] = sc[2 * nk + i / 2][0], (&z)[4] = sc[2 * nk + i / 2][1];
-                    float x = (y[i % 2] + z[i % 2]) + (y[2 + i % 2] + z[2 + i % 2]);
-                    if constexpr (THREE) x += __shfl_xor_sync(0xffffffffu, x, 16);
-                    x *= unit;
-                    if constexpr (E4M3) x *= scales[t];
-                    w[nk][i] = seen >> t & 1u ? x : -INFINITY;
-                    top = fmaxf(top, w[nk][i]);
-                    if constexpr (E4M3) {       // a value's scale goes into its weight: 2^e, e from the exponent field
-                        vs[nk][i] = w[nk][i] + (float)((int)(__float_as_uint(scales[TOKENS + t]) >> 23) - 127);
-                        topv = fmaxf(topv, vs[nk][i]);
-                    }
+            for (int i = 0; i < 2 * NK; ++i) {
+                const float (&y)[4] = sc[i][0], (&z)[4] = sc[i][1];
+                float2 x = unpair(add2(add2(pair(y[0], y[1]), pair(z[0], z[1])), add2(pair(y[2], y[3]), pair(z[2], z[3]))));
+                if constexpr (THREE) {
+                    x.x += __shfl_xor_sync(0xffffffffu, x.x, 16);
+                    x.y += __shfl_xor_sync(0xffffffffu, x.y, 16);
                 }
+                x.x *= unit;
+                x.y *= unit;
+                if constexpr (E4M3) {
+                    const float2 k = *reinterpret_cast<const float2*>(scales + 8 * i + 2 * r);
+                    x.x *= k.x;
+                    x.y *= k.y;
+                }
+                w[i / 2][i % 2 * 2] = x.x;
+                w[i / 2][i % 2 * 2 + 1] = x.y;
+            }
+            if (seen != 0xffffffffu >> (32 - TOKENS)) {
+#pragma unroll
+                for (int i = 0; i < 4 * NK; ++i) w[i / 4][i % 4] = seen >> (i / 2 * 8 + 2 * r + i % 2) & 1u ? w[i / 4][i % 4] : -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < 4 * NK; ++i) {
+                top = fmaxf(top, w[i / 4][i % 4]);
+                if constexpr (E4M3) {           // a value's scale goes into its weight: 2^e, e from the exponent field
+                    vs[i / 4][i % 4] = w[i / 4][i % 4] + (float)((int)(__float_as_uint(scales[TOKENS + i / 2 * 8 + 2 * r + i % 2]) >> 23) - 127);
+                    topv = fmaxf(topv, vs[i / 4][i % 4]);
+                }
+            }
             // ---- weights
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -533,8 +565,10 @@ struct TensorWarp {
                 }
             }
             // ---- values
+            const unsigned long long keep2 = pair(keep, keep);
 #pragma unroll
             for (int c = 0; c < VC; ++c) {
+                if (!PACKED && c > 0 && c * 8 * VE >= width) break;
                 unsigned x[NK][4][4];
 #pragma unroll
                 for (int nk = 0; nk < NK; ++nk)
@@ -571,10 +605,10 @@ struct TensorWarp {
                             }
                         }
                         if constexpr (E4M3) {
-                            add(c * VE + 4 * i + 2 * e, y0, keep);
-                            add(c * VE + 4 * i + 2 * e + 1, y1, keep);
+                            add(c * VE + 4 * i + 2 * e, y0, keep2);
+                            add(c * VE + 4 * i + 2 * e + 1, y1, keep2);
                         } else {
-                            add(c * VE + 2 * i + e, y0, keep);
+                            add(c * VE + 2 * i + e, y0, keep2);
                         }
                     }
             }
@@ -589,11 +623,10 @@ struct TensorWarp {
         const float back = E4M3 ? exp2_of(settled(mv) - settled(m) - LIFT) : 1.0f;
 #pragma unroll
         for (int i = 0; i < VC * VE; ++i) {
-            acc[i][0] *= back;
-            acc[i][1] *= back;
+            if constexpr (E4M3) acc[i] = mul2(acc[i], pair(back, back));
             if constexpr (THREE) {
-                acc[i][0] += __shfl_xor_sync(0xffffffffu, acc[i][0], 16);
-                acc[i][1] += __shfl_xor_sync(0xffffffffu, acc[i][1], 16);
+                const float2 x = unpair(acc[i]);
+                acc[i] = pair(x.x + __shfl_xor_sync(0xffffffffu, x.x, 16), x.y + __shfl_xor_sync(0xffffffffu, x.y, 16));
             }
         }
     }
@@ -608,8 +641,9 @@ struct TensorWarp {
 #pragma unroll
             for (int j = 0; j < VE; ++j) {
                 float* at = out + g * DP + c * 8 * VE + 2 * r * VE + j;
-                at[0] = acc[c * VE + j][0];
-                at[VE] = acc[c * VE + j][1];
+                const float2 x = unpair(acc[c * VE + j]);
+                at[0] = x.x;
+                at[VE] = x.y;
             }
     }
 };
@@ -659,6 +693,7 @@ struct FmaWarp {
     float m[OWN], l[OWN];          // of heads r, r + 4 (modulo HT); l over this lane's tokens only
 
     float unit;                    // what a score is multiplied by
+    int width;                     // d: !PACKED pieces behind it are left out
 
     __device__ __forceinline__ void begin(const AttnParams& p, const float*) {
 #pragma unroll
@@ -668,6 +703,7 @@ struct FmaWarp {
 #pragma unroll
         for (int i = 0; i < OWN; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
         unit = p.scale * LOG2E;
+        width = p.d;
     }
 
     __device__ __forceinline__ void step(const char* keys, unsigned seen, unsigned* words) {
@@ -687,6 +723,7 @@ struct FmaWarp {
                 for (int h = 0; h < HT; ++h) part[h][0] = part[h][1] = 0ull;
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {
+                    if (!PACKED && c * 16 >= width) break;
                     const ulonglong2 kk = *reinterpret_cast<const ulonglong2*>(keys + R::key_at(g + 8 * i, 4 * c + r));
 #pragma unroll
                     for (int h = 0; h < HT; ++h) {
@@ -864,7 +901,7 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
         total += scan[i];
     }
     const int units = total * tiles_of_heads;
-    const Shares shares = shares_of(units, max(1, min(units, (int)gridDim.x)));       // every worker has a unit
+    const Shares shares = shares_of(units, max(1, min(units / (DTYPE == TE_KV_F32 ? 1 : 2), (int)gridDim.x)));     // every worker has a unit, or two
     const int unit = w < shares.workers ? share_begin(shares, w) : 0;
     const int unit_end = w < shares.workers ? share_begin(shares, w + 1) : 0;
     if (unit < unit_end) {
