@@ -473,8 +473,10 @@ TE_API int te_b200_kv_read(te_b200_ctx* ctx, const te_kv_desc* d, te_stream_t st
  * zeros and -infinity.  Cached tokens outside the range are never read.  Rows may share pages, or whole rows of the table
  * (page_table_stride 0): several tokens of one sequence are rows with growing lens.  lens beyond
  * max_pages * page_size is cut to it, and a page outside [0, pages) counts as masked; both are reported by
- * te_b200_check_device_status.  Softmax statistics and sums are kept in FP32 and joined in a fixed order.
- * Uses the context workspace. */
+ * te_b200_check_device_status.  Softmax statistics and sums are kept in FP32 and joined in a fixed order, so two calls
+ * give the same bits.  A query, key or value that is not finite makes the results that it enters not finite.
+ * max_pages * page_size is at most 2^31 - 4097.  Uses the context workspace and its counters, so calls of one context follow one
+ * another on one stream, captured ones included. */
 typedef struct te_paged_attn_desc {
     te_kv_cache cache;
     int64_t rows, q_heads;

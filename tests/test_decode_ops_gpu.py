@@ -255,12 +255,15 @@ def test_cache_refusals(backend):
 class Scene:
     """Rows of the given lengths in a cache whose unused places hold NaN, and the exact answers."""
 
-    def __init__(self, dtype, lengths, hq, hk, d, page, seed=0, order="phsd", spread=1.0):
+    def __init__(self, dtype, lengths, hq, hk, d, page, seed=0, order="phsd", spread=1.0, value_order=None):
         self.dtype, self.lengths, self.hq, self.hk, self.d, self.page = dtype, lengths, hq, hk, d, page
         self.pages = sum(-(-n // page) for n in lengths) + 3
         self.table = scattered(lengths, page, self.pages, seed)
         longest = max(1, max(lengths))
         self.cache = make_cache(dtype, self.pages, hk, page, d, order, fill=0xff)      # all bits set: NaN in every type
+        if value_order:
+            other = make_cache(dtype, self.pages, hk, page, d, value_order, fill=0xff)
+            self.cache = ops.KvCache(self.cache.k, other.v, self.cache.k_scale, self.cache.v_scale)
         k, v = normal(seed + 1, len(lengths), hk, longest, d) * spread, normal(seed + 2, len(lengths), hk, longest, d)
         self.q = normal(seed + 3, len(lengths), hq, d) * 1.5
         at = torch.arange(longest).expand(len(lengths), -1)
@@ -315,6 +318,31 @@ def test_attention(backend, dtype, lengths, hq, hk, d, page, order):
     scene.check(o, lse)
     o2, lse2 = scene.run(backend)
     assert torch.equal(o, o2) and torch.equal(lse, lse2), "two runs differ"
+    backend.check_device_status()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "e4m3"])
+@pytest.mark.parametrize("d,page", [(64, 16), (80, 16), (128, 7)])
+def test_attention_with_keys_and_values_in_different_orders(backend, dtype, d, page):
+    scene = Scene(dtype, [90, 33, 0, 200], 6, 2, d, page, order="phsd", value_order="pshd").fill(backend)
+    scene.check(*scene.run(backend))
+    scene = Scene(dtype, [90, 33, 0, 200], 6, 2, d, page, order="hpsd", value_order="phsd").fill(backend)
+    scene.check(*scene.run(backend))
+    backend.check_device_status()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "e4m3"])
+def test_attention_of_many_rows(backend, dtype):
+    """More rows than a block has threads, some empty, one long among short ones; a sample of the rows is checked."""
+    lengths = [(37 * r) % 90 for r in range(300)]
+    lengths[123], lengths[299] = 2600, 0
+    scene = Scene(dtype, lengths, 4, 2, 64, 16).fill(backend)
+    o, lse = scene.run(backend)
+    scene.check(o, lse, rows=[0, 1, 2, 90, 122, 123, 124, 127, 128, 129, 180, 255, 256, 298, 299])
+    o2, _ = scene.run(backend)
+    assert torch.equal(o, o2)
+    # each row alone gives the same within the bounds: no row reads another's share
+    assert bool(torch.isfinite(o).all())
     backend.check_device_status()
 
 
@@ -408,6 +436,11 @@ def test_attention_without_pages(backend):
     assert bool((o == 0).all()) and bool((lse == -math.inf).all())
     assert backend.paged_attention(q[:0], cache, table[:0], lens[:0]).shape == (0, 4, 64)
     backend.check_device_status()
+    # lengths and page numbers where there are no pages: masked and reported
+    o, lse = backend.paged_attention(q, cache, torch.zeros(2, 3, dtype=torch.int64, device="cuda"), lens + 5, want_lse=True)
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+    with pytest.raises(L.BackendError):
+        backend.check_device_status()
 
 
 def test_attention_beyond_32_bit_offsets(backend):
@@ -430,6 +463,16 @@ def test_attention_beyond_32_bit_offsets(backend):
         bound, bound_lse = ref.attention_bound(d, n, absolute, top, reach)
         within(o[0, h:h + 1], want, bound)
         within(lse[0, h:h + 1], want_lse, bound_lse)
+
+
+def test_attention_needs_its_workspace(backend):
+    small = ops.Backend(0, workspace_bytes=4096)
+    cache = small.kv_cache(4, 2, 8, 32, "f32")
+    q, table, lens = torch.zeros(1, 4, 32, device="cuda"), torch.zeros(1, 2, dtype=torch.int64, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+    with pytest.raises(L.BackendError) as e:
+        small.paged_attention(q, cache, table, lens)
+    assert e.value.status == L.TE_ERR_WORKSPACE
+    small.close()
 
 
 def test_attention_refusals(backend):

@@ -38,10 +38,12 @@ constexpr int THREADS = 32 * WARPS;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
-// Thread blocks per SM, a power of the registers and the rings: three with two stages each where 168 registers a thread will do
-// and two stages of a block's four warps take at most 66 KB, else two with three stages, one for the longest rows.
+// Thread blocks per SM, as registers and rings allow.  bf16 rows of up to 256 bytes and FP32 tiles of one or two heads do with 168
+// registers a thread, so three blocks with two stages each (window of 4096 bf16 tokens: 48 us against 52 with two blocks
+// of three stages).  e4m3 spills at 168 (two 131072-token rows: 75 us against 74), wide FP32 tiles too: two blocks.  Two rings of
+// the longest rows do not fit: one block.
 constexpr int blocks_per_sm(int dtype, int d, int heads) {
-    return dtype == TE_KV_E4M3 ? (d <= 128 ? 3 : 2) : d > 128 ? 1 : dtype == TE_KV_BF16 || heads <= 2 ? 3 : 2;
+    return dtype == TE_KV_E4M3 ? 2 : d > 128 ? 1 : dtype == TE_KV_BF16 || heads <= 2 ? 3 : 2;
 }
 
 struct AttnParams {
@@ -1219,7 +1221,7 @@ int te_b200_paged_attention(te_b200_ctx* ctx, const te_paged_attn_desc* t, te_st
     for (int i = 0; i < 3; ++i) { p.kcs[i] = c.k_strides[i] * size; p.vcs[i] = c.v_strides[i] * size; p.ss[i] = c.scale_strides[i]; }
     p.table_stride = t->page_table_stride; p.pages = c.pages; p.window = t->window;
     p.page_size = make_fast_divisor((uint32_t)c.page_size);
-    p.most = (int)(t->max_pages * c.page_size);
+    p.most = c.pages > 0 ? (int)(t->max_pages * c.page_size) : 0;      // (a cache without pages has no places)
     p.q_heads = (int)t->q_heads; p.kv_heads = (int)c.heads;
     p.group = (int)(t->q_heads / c.heads); p.d = (int)c.d;
     const int heads = heads_per_tile(c.dtype, p.group);
