@@ -9,6 +9,7 @@
 //   te::ScaledDot       softmax(Q.K^T / sqrt(d)).V and its backward        (reference src/nn/scaledot.cpp:8-27)
 //   te::LayerNorm, te::Embedding, te::cross_entropy: the GPT step's kernels around the matmuls
 //                       (reference src/nn/layernorm.cpp, src/nn/embedding.cpp, src/loss/CrossEntropyLoss.cpp)
+//   te::Rotary, te::KvCache, te::paged_attention: answering token by token (no reference counterpart)
 // Errors surface as std::runtime_error with the reference's texts (src/tensor/tensor.h:537, :547, :626, :858).
 // Tensors live on the GPU only: this backend has no CPU compute path.  Each Tensor owns (or shares) one device
 // buffer from te::CachingAllocator (the reference's CUDAAllocator calls cudaMalloc per tensor, src/core/allocators.h:35-52).
@@ -18,6 +19,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <cstdint>
+#include <cstring>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -601,6 +603,119 @@ inline Tensor cross_entropy(const Tensor& logits, const IndexArray& targets, Ten
     check(te_b200_cross_entropy(be.ctx(), logits.data(), targets.data(), loss.data(), dlogits ? grad.data() : nullptr, 1.0f, rows, V, current_stream()));
     if (dlogits) *dlogits = grad;
     return loss;
+}
+
+// Rotary positions of the first `rot` elements of every head (te_b200_rotary); scaling is a TE_ROTARY_* value.
+class Rotary {
+public:
+    explicit Rotary(int64_t rot, double base = 10000.0, int scaling = TE_ROTARY_PLAIN, double factor = 1.0, int64_t trained_length = 0,
+                    double slow_turns = 1.0, double fast_turns = 32.0, bool interleaved = false, float scale = 1.0f)
+        : rot_(rot), interleaved_(interleaved), scale_(scale), inv_freq_(frequencies(rot, base, scaling, factor, trained_length, slow_turns, fast_turns)) {}
+    // x [B,H,T,d], any view with a unit last stride; positions: B * T.
+    Tensor forward(const Tensor& x, const IndexArray& positions) const { return turn(x, positions, 0); }
+    Tensor backward(const Tensor& dy, const IndexArray& positions) const { return turn(dy, positions, 1); }
+private:
+    // (the 64-bit device array holds the frequencies' bit patterns)
+    static IndexArray frequencies(int64_t rot, double base, int scaling, double factor, int64_t trained_length, double slow_turns, double fast_turns) {
+        std::vector<double> f((size_t)(rot > 0 ? rot / 2 : 0));
+        check(te_b200_rotary_inv_freq(rot, base, scaling, factor, trained_length, slow_turns, fast_turns, f.data()));
+        std::vector<int64_t> bits(f.size());
+        if (!f.empty()) std::memcpy(bits.data(), f.data(), f.size() * sizeof(double));
+        return IndexArray(bits);
+    }
+    Tensor turn(const Tensor& x, const IndexArray& positions, int inverse) const {
+        if (x.shape().size() != 4) throw std::runtime_error("Rotary expects a [B, H, T, d] view");
+        const int64_t B = x.shape()[0], H = x.shape()[1], T = x.shape()[2], d = x.shape()[3];
+        if (x.strides()[3] != 1 && d > 1) throw std::runtime_error("Rotary: the last dimension must have unit stride");
+        if ((int64_t)positions.size() != B * T) throw std::runtime_error("Rotary: one position per token [B, T]");
+        Tensor y({B, H, T, d});
+        te_rotary_desc r = {};
+        r.B = B; r.H = H; r.T = T; r.d = d; r.rot = rot_;
+        r.x = x.data(); r.y = y.data();
+        for (int i = 0; i < 3; ++i) { r.x_strides[i] = x.strides()[i]; r.y_strides[i] = y.strides()[i]; }
+        r.positions = positions.data(); r.position_strides[0] = T; r.position_strides[1] = 1;
+        r.inv_freq = reinterpret_cast<const double*>(inv_freq_.data());
+        r.scale = scale_; r.interleaved = interleaved_; r.inverse = inverse;
+        check(te_b200_rotary(Backend::instance().ctx(), &r, current_stream()));
+        return y;
+    }
+    int64_t rot_;
+    bool interleaved_;
+    float scale_;
+    IndexArray inv_freq_;
+};
+
+// Keys and values in pages, [pages, heads, page_size, d] (te_kv_cache); dtype is a TE_KV_* value.  page_table: rows of max_pages
+// page numbers, one per sequence; positions: one per token, negative for padding.
+class KvCache {
+public:
+    KvCache(int64_t pages, int64_t heads, int64_t page_size, int64_t d, int dtype = TE_KV_F32) {
+        if (pages < 0 || heads < 0 || page_size < 1 || d < 1) throw std::runtime_error("KvCache: bad extents");
+        if (dtype < TE_KV_F32 || dtype > TE_KV_E4M3) throw std::runtime_error("KvCache: dtype must be a TE_KV_* value");
+        desc_.pages = pages; desc_.heads = heads; desc_.page_size = page_size; desc_.d = d; desc_.dtype = dtype;
+        const int64_t page = heads * page_size * d, slots = heads * page_size, size = dtype == TE_KV_F32 ? 4 : dtype == TE_KV_BF16 ? 2 : 1;
+        const int64_t strides[3] = {page, page_size * d, d}, scale_strides[3] = {slots, page_size, 1};
+        for (int i = 0; i < 3; ++i) { desc_.k_strides[i] = desc_.v_strides[i] = strides[i]; desc_.scale_strides[i] = scale_strides[i]; }
+        const size_t side = ((size_t)(pages * page * size) + 255) & ~size_t(255), scales = dtype == TE_KV_E4M3 ? ((size_t)(pages * slots * 4) + 255) & ~size_t(255) : 0;
+        size_t block = 0;
+        char* p = static_cast<char*>(CachingAllocator::instance().allocate(2 * side + 2 * scales + 256, &block));
+        storage_ = std::shared_ptr<void>(p, [block](void* q) { CachingAllocator::instance().release(q, block); });
+        desc_.k = p; desc_.v = p + side;
+        if (scales) { desc_.k_scale = reinterpret_cast<float*>(p + 2 * side); desc_.v_scale = reinterpret_cast<float*>(p + 2 * side + scales); }
+    }
+    const te_kv_cache& desc() const { return desc_; }
+    // k, v: [B, heads, T, d], any views with a unit last stride.
+    void append(const Tensor& k, const Tensor& v, const IndexArray& page_table, int64_t max_pages, const IndexArray& positions) {
+        te_kv_desc m = move(k, v, page_table, max_pages, positions);
+        check(te_b200_kv_append(Backend::instance().ctx(), &m, current_stream()));
+    }
+    // {k, v} [B, heads, T, d] of the tokens at these positions (B * T of them), zeros at negative ones.
+    std::vector<Tensor> read(const IndexArray& page_table, int64_t max_pages, const IndexArray& positions, int64_t B, int64_t T) const {
+        Tensor k({B, desc_.heads, T, desc_.d}), v({B, desc_.heads, T, desc_.d});
+        te_kv_desc m = move(k, v, page_table, max_pages, positions);
+        check(te_b200_kv_read(Backend::instance().ctx(), &m, current_stream()));
+        return {k, v};
+    }
+private:
+    te_kv_desc move(const Tensor& k, const Tensor& v, const IndexArray& page_table, int64_t max_pages, const IndexArray& positions) const {
+        if (k.shape().size() != 4 || k.shape() != v.shape() || k.shape()[1] != desc_.heads || k.shape()[3] != desc_.d)
+            throw std::runtime_error("KvCache expects k and v [B, heads, T, d]");
+        if (k.strides()[3] != 1 || v.strides()[3] != 1) throw std::runtime_error("KvCache: the last dimension must have unit stride");
+        te_kv_desc m = {};
+        m.cache = desc_;
+        m.B = k.shape()[0]; m.T = k.shape()[2];
+        if ((int64_t)page_table.size() != m.B * max_pages || (int64_t)positions.size() != m.B * m.T)
+            throw std::runtime_error("KvCache: a row of max_pages page numbers per sequence and one position per token");
+        m.k = k.data(); m.v = v.data();
+        for (int i = 0; i < 3; ++i) { m.k_strides[i] = k.strides()[i]; m.v_strides[i] = v.strides()[i]; }
+        m.page_table = page_table.data(); m.page_table_stride = max_pages; m.max_pages = max_pages;
+        m.positions = positions.data(); m.position_strides[0] = m.T; m.position_strides[1] = 1;
+        return m;
+    }
+    te_kv_cache desc_ = {};
+    std::shared_ptr<void> storage_;
+};
+
+// Attention of one new token per row, q [rows, q_heads, d], over the first lens[row] cached tokens of the row's sequence (the last
+// `window` of them if window > 0), scaled by 1 / sqrt(d); lse (optional) receives the log-sum-exp [rows, q_heads].
+inline Tensor paged_attention(const Tensor& q, const KvCache& cache, const IndexArray& page_table, int64_t max_pages, const IndexArray& lens,
+                              int64_t window = 0, Tensor* lse = nullptr) {
+    if (q.shape().size() != 3 || q.shape()[2] != cache.desc().d || q.strides()[2] != 1)
+        throw std::runtime_error("paged_attention expects q [rows, q_heads, d] with the cache's d and a unit last stride");
+    te_paged_attn_desc a = {};
+    a.cache = cache.desc();
+    a.rows = q.shape()[0]; a.q_heads = q.shape()[1];
+    if ((int64_t)page_table.size() != a.rows * max_pages || (int64_t)lens.size() != a.rows)
+        throw std::runtime_error("paged_attention: a row of max_pages page numbers and one length per row");
+    Tensor o(q.shape());
+    if (lse) *lse = Tensor({a.rows, a.q_heads});
+    a.q = q.data(); a.o = o.data(); a.lse = lse ? lse->data() : nullptr;
+    for (int i = 0; i < 2; ++i) { a.q_strides[i] = q.strides()[i]; a.o_strides[i] = o.strides()[i]; }
+    a.page_table = page_table.data(); a.page_table_stride = max_pages; a.max_pages = max_pages; a.lens = lens.data();
+    a.window = window;
+    a.scale = 1.0f / std::sqrt((float)cache.desc().d);
+    check(te_b200_paged_attention(Backend::instance().ctx(), &a, current_stream()));
+    return o;
 }
 
 }  // namespace te
