@@ -8,6 +8,9 @@
 // side by side in the cache's usual order [pages, heads, page_size, d], and their positions, page numbers and data are
 // three loads one after the other that ROWS tokens wait for together.  Each lane works out the place of one of these
 // tokens and the others take it from there.
+//
+// Measured (share of the 6.54 TB/s of a copy): FP32 [64,6,256,64] 18.0 us, 85 %; padded prompts [8,8,2001,128] into bf16 15.2 us,
+// 79 % of what is not padding; [4,8,4093,128] into e4m3 and back 46 us, 79 %; 64 tokens of 8 heads 1.7 us, a launch's latency.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
@@ -223,8 +226,9 @@ __global__ void __launch_bounds__(256) kv_move_kernel(const KvParams p) {
     }
 }
 
-// Tokens a group moves at once: one where there are few per sequence; else two rows of FP32 in and out, or up to four (written)
-// or eight (read) of the narrower types.
+// Tokens a group moves at once: one where there are few per sequence; else two rows of FP32 in and out (17.5 us for
+// [64,6,256,64], 17.9 with four), or up to four (written; padded bf16 prompts 15.2 us, 16.2 with two) or eight (read) of the
+// narrower types.
 constexpr int MOST_F32 = 2, MOST_APPENDED = 4, MOST_READ = 8;
 int rows_at_once(int dtype, int T, int d, bool append) {
     if (T < 4) return 1;
