@@ -568,6 +568,59 @@ def test_captured_steps_replay_with_new_contents(backend, dtype):
     backend.check_device_status()
 
 
+def test_two_captured_graphs_share_the_workspace_one_after_the_other(backend):
+    """Graphs of two scenes captured from one backend (one joins inside, one by the second kernel), replayed in turn with eager calls
+    between them."""
+    scenes = [Scene("bf16", [700, 0, 1500, 33], 8, 2, 64, 16).fill(backend), Scene("f32", [6000], 1, 1, 64, 16, seed=9).fill(backend)]
+    want = [s.run(backend) for s in scenes]
+    graphs, outs = [], []
+    for s in scenes:
+        q, table, lens = s.q.cuda(), s.table.cuda(), torch.tensor(s.lengths).cuda()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(backend.paged_attention(q, s.cache, table, lens, want_lse=True))
+        graphs.append((graph, q, table, lens))
+    for turn in range(6):
+        for i in (0, 1, 1, 0):
+            for t in outs[i]:
+                t.zero_()
+            graphs[i][0].replay()
+            again = scenes[1 - i].run(backend)
+            assert torch.equal(outs[i][0], want[i][0]) and torch.equal(outs[i][1], want[i][1]), (turn, i)
+            assert torch.equal(again[0], want[1 - i][0])
+    backend.check_device_status()
+
+
+def test_captured_before_any_other_call():
+    """A context's first calls may be captured ones: a process of its own, whose first use of these kernels is in a capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch
+from torch_engine_b200 import ops
+be = ops.Backend(0, workspace_bytes=64 << 20)
+x = torch.ones(2, 3, 1, 64, device="cuda")
+table, pos, lens = torch.zeros(2, 1, dtype=torch.int64, device="cuda"), torch.zeros(2, 1, dtype=torch.int64, device="cuda"), torch.ones(2, dtype=torch.int64, device="cuda")
+table[1] = 1
+cache, f = be.kv_cache(2, 1, 16, 64, "bf16"), be.rotary_inv_freq(64)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = be.rotary(x, pos, f)
+    be.kv_append(cache, y[:, 1:2], y[:, 2:], table, pos)
+    o = be.paged_attention(y[:, :1, 0], cache, table, lens)
+g.replay()
+be.check_device_status()
+assert torch.equal(o, torch.ones(2, 1, 64, device="cuda")), o
+print("captured first")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
+
+
 def test_on_another_stream_and_a_context_of_its_own(backend):
     """Two backends on two streams at once: each has its own workspace."""
     other = ops.Backend(0, workspace_bytes=64 << 20)
