@@ -8,15 +8,16 @@
 // * A fixed number of thread blocks, all resident, share the tiles of all rows evenly (paged_plan.h), so that one long
 //   sequence, many short ones and any mixture keep every SM reading.  A block that holds only part of a (row, head tile)
 //   leaves its sums in the workspace; paged_join_kernel adds the parts in their order.
-// * Every warp copies its own tokens into a ring of its own in shared memory, 16 bytes a lane with cp.async, two stages
-//   ahead of the one it computes on, and waits for nobody else until the segment ends.
+// * Every warp copies its own tokens into a ring of its own in shared memory, 16 bytes a lane with cp.async, one or two stages
+//   ahead of the one it computes on and on into its next segments, and waits for nobody else until a segment ends.
 //
 // 2- and 1-byte caches use the tensor cores through mma.sync m16n8k16 (8 query rows do not fill the 128-row tiles of
-// tcgen05, and the products need 5 % of the tensor rate): a stored value is exactly a bf16 resp. half, and an FP32 query
-// or weight is exactly (to 2^-24 of its row's largest) the sum of three bf16 resp. two half terms, so that products and
-// sums are those of FP32 (relative error against 64 bits 2e-7 to 4e-7).  The terms of a head occupy rows g and g + 8 of one tile, both in the same thread.  Which element of a head
-// an index of the contraction stands for is free as long as both operands agree, and chosen so that a lane's operand is 16
-// bytes of a row as it lies in the cache.  An FP32 cache uses FP32 FMAs (two per instruction).
+// tcgen05, and the tensor pipe is 20 to 35 % busy): a stored value is exactly a bf16 resp. half, and an FP32 query or
+// weight is, to 2^-24 of its row's largest, the sum of three bf16 resp. two half terms, so that products and sums are
+// those of FP32 (relative error against 64 bits 2e-7 to 4e-7).  The terms of a head occupy rows g and g + 8 of one tile,
+// both in the same thread.  Which element of a head an index of the contraction stands for is free as long as both
+// operands agree, and chosen so that a lane's operand is 16 bytes of a row as it lies in the cache.  An FP32 cache uses
+// FP32 FMAs (two per instruction).
 //
 // Measured (device time, share of the 6.54 TB/s of a copy): 32 rows of 164 to 16384 tokens, 32 query and 8 key heads of 128,
 // bf16: 86 us, 94 %; two rows of up to 131072 tokens, 64/8 heads, e4m3: 74 us, 82 % (bound by instruction issue: every
@@ -459,167 +460,165 @@ struct TensorWarp {
         const int lane = threadIdx.x % 32, g = lane / 4, r = lane % 4;
         const char* values = keys + R::SIDE;
         const float* scales = reinterpret_cast<const float*>(keys + 2 * R::SIDE);
-        {
-            // ---- scores
-            // (two chains of products for every 8 tokens: a product waits for the one before it in its chain)
-            float sc[2 * NK][2][4];
+        // ---- scores
+        // (two chains of products for every 8 tokens: a product waits for the one before it in its chain)
+        float sc[2 * NK][2][4];
 #pragma unroll
-            for (int c = 0; c < KG; ++c) {
-                if (!PACKED && c > 0 && c * (4 * 16 / ES) >= width) break;
-                const uint4* q = reinterpret_cast<const uint4*>(words) + c * KQ * 32 + lane;
-                uint4 qw[KQ];
+        for (int c = 0; c < KG; ++c) {
+            if (!PACKED && c > 0 && c * (4 * 16 / ES) >= width) break;
+            const uint4* q = reinterpret_cast<const uint4*>(words) + c * KQ * 32 + lane;
+            uint4 qw[KQ];
 #pragma unroll
-                for (int i = 0; i < KQ; ++i) qw[i] = q[32 * i];
+            for (int i = 0; i < KQ; ++i) qw[i] = q[32 * i];
 #pragma unroll
-                for (int i = 0; i < 2 * NK; ++i) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(keys + R::key_at(i * 8 + g, 4 * c + r));
-                    float (&y)[4] = sc[i][0], (&z)[4] = sc[i][1];
-                    if constexpr (E4M3) {
-                        const uint2 k0 = halves_of_e4m3(x.x), k1 = halves_of_e4m3(x.y), k2 = halves_of_e4m3(x.z), k3 = halves_of_e4m3(x.w);
-                        mma_first_or_next<true>(c == 0, y, qw[0], k0.x, k0.y);
-                        mma_first_or_next<true>(c == 0, z, qw[1], k1.x, k1.y);
-                        mma<true>(y, qw[2], k2.x, k2.y);
-                        mma<true>(z, qw[3], k3.x, k3.y);
-                    } else {
-                        mma_first_or_next<false>(c == 0, y, qw[0], x.x, x.y);
-                        mma_first_or_next<false>(c == 0, z, qw[1], x.z, x.w);
-                        if constexpr (!THREE) {
-                            mma<false>(y, qw[2], x.x, x.y);
-                            mma<false>(z, qw[3], x.z, x.w);
-                        }
+            for (int i = 0; i < 2 * NK; ++i) {
+                const uint4 x = *reinterpret_cast<const uint4*>(keys + R::key_at(i * 8 + g, 4 * c + r));
+                float (&y)[4] = sc[i][0], (&z)[4] = sc[i][1];
+                if constexpr (E4M3) {
+                    const uint2 k0 = halves_of_e4m3(x.x), k1 = halves_of_e4m3(x.y), k2 = halves_of_e4m3(x.z), k3 = halves_of_e4m3(x.w);
+                    mma_first_or_next<true>(c == 0, y, qw[0], k0.x, k0.y);
+                    mma_first_or_next<true>(c == 0, z, qw[1], k1.x, k1.y);
+                    mma<true>(y, qw[2], k2.x, k2.y);
+                    mma<true>(z, qw[3], k3.x, k3.y);
+                } else {
+                    mma_first_or_next<false>(c == 0, y, qw[0], x.x, x.y);
+                    mma_first_or_next<false>(c == 0, z, qw[1], x.z, x.w);
+                    if constexpr (!THREE) {
+                        mma<false>(y, qw[2], x.x, x.y);
+                        mma<false>(z, qw[3], x.z, x.w);
                     }
                 }
             }
-            float w[NK][4], vs[NK][4];
-            float top = -INFINITY, topv = -INFINITY;
+        }
+        float w[NK][4], vs[NK][4];
+        float top = -INFINITY, topv = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2 * NK; ++i) {
-                const float (&y)[4] = sc[i][0], (&z)[4] = sc[i][1];
-                float2 x = unpair(add2(add2(pair(y[0], y[1]), pair(z[0], z[1])), add2(pair(y[2], y[3]), pair(z[2], z[3]))));
-                if constexpr (THREE) {
-                    x.x += __shfl_xor_sync(0xffffffffu, x.x, 16);
-                    x.y += __shfl_xor_sync(0xffffffffu, x.y, 16);
-                }
-                x.x *= unit;
-                x.y *= unit;
-                if constexpr (E4M3) {
-                    const float2 k = *reinterpret_cast<const float2*>(scales + 8 * i + 2 * r);
-                    x.x *= k.x;
-                    x.y *= k.y;
-                }
-                w[i / 2][i % 2 * 2] = x.x;
-                w[i / 2][i % 2 * 2 + 1] = x.y;
+        for (int i = 0; i < 2 * NK; ++i) {
+            const float (&y)[4] = sc[i][0], (&z)[4] = sc[i][1];
+            float2 x = unpair(add2(add2(pair(y[0], y[1]), pair(z[0], z[1])), add2(pair(y[2], y[3]), pair(z[2], z[3]))));
+            if constexpr (THREE) {
+                x.x += __shfl_xor_sync(0xffffffffu, x.x, 16);
+                x.y += __shfl_xor_sync(0xffffffffu, x.y, 16);
             }
-            if (seen != 0xffffffffu >> (32 - TOKENS)) {
+            x.x *= unit;
+            x.y *= unit;
+            if constexpr (E4M3) {
+                const float2 k = *reinterpret_cast<const float2*>(scales + 8 * i + 2 * r);
+                x.x *= k.x;
+                x.y *= k.y;
+            }
+            w[i / 2][i % 2 * 2] = x.x;
+            w[i / 2][i % 2 * 2 + 1] = x.y;
+        }
+        if (seen != 0xffffffffu >> (32 - TOKENS)) {
 #pragma unroll
-                for (int i = 0; i < 4 * NK; ++i) w[i / 4][i % 4] = seen >> (i / 2 * 8 + 2 * r + i % 2) & 1u ? w[i / 4][i % 4] : -INFINITY;
-            }
+            for (int i = 0; i < 4 * NK; ++i) w[i / 4][i % 4] = seen >> (i / 2 * 8 + 2 * r + i % 2) & 1u ? w[i / 4][i % 4] : -INFINITY;
+        }
 #pragma unroll
-            for (int i = 0; i < 4 * NK; ++i) {
-                top = fmaxf(top, w[i / 4][i % 4]);
-                if constexpr (E4M3) {           // a value's scale goes into its weight: 2^e, e from the exponent field
-                    vs[i / 4][i % 4] = w[i / 4][i % 4] + (float)((int)(__float_as_uint(scales[TOKENS + i / 2 * 8 + 2 * r + i % 2]) >> 23) - 127);
-                    topv = fmaxf(topv, vs[i / 4][i % 4]);
+        for (int i = 0; i < 4 * NK; ++i) {
+            top = fmaxf(top, w[i / 4][i % 4]);
+            if constexpr (E4M3) {           // a value's scale goes into its weight: 2^e, e from the exponent field
+                vs[i / 4][i % 4] = w[i / 4][i % 4] + (float)((int)(__float_as_uint(scales[TOKENS + i / 2 * 8 + 2 * r + i % 2]) >> 23) - 127);
+                topv = fmaxf(topv, vs[i / 4][i % 4]);
+            }
+        }
+        // ---- weights
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = fmaxf(top, m);
+        const float base = settled(top);
+        float keep = exp2_of(m - base), sum = 0.0f;
+#pragma unroll
+        for (int nk = 0; nk < NK; ++nk)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = exp2_of(w[nk][i] - base);
+                sum += e;
+                if constexpr (!E4M3) w[nk][i] = e;
+            }
+        l = l * keep + sum;
+        m = top;
+        if constexpr (E4M3) {
+            topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 1));
+            topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 2));
+            topv = fmaxf(topv, mv);
+            const float basev = settled(topv);
+            keep = exp2_of(mv - basev);
+#pragma unroll
+            for (int nk = 0; nk < NK; ++nk)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[nk][i] = exp2_of(vs[nk][i] - basev + LIFT);
+            mv = topv;
+        }
+        uint4 a[NK], lower[NK];         // left operands of P; bf16: the lowest terms apart
+#pragma unroll
+        for (int nk = 0; nk < NK; ++nk) {
+            float x0 = w[nk][0], x1 = w[nk][1], x2 = w[nk][2], x3 = w[nk][3];
+            if constexpr (E4M3) {
+                a[nk].x = pack_half(x0, x1);
+                a[nk].z = pack_half(x2, x3);
+                const float2 f = unpack_half(a[nk].x), h = unpack_half(a[nk].z);
+                a[nk].y = pack_half(x0 - f.x, x1 - f.y);
+                a[nk].w = pack_half(x2 - h.x, x3 - h.y);
+            } else {
+                a[nk].x = pack_bf16(x0, x1);
+                a[nk].z = pack_bf16(x2, x3);
+                x0 -= bf16_lo(a[nk].x); x1 -= bf16_hi(a[nk].x); x2 -= bf16_lo(a[nk].z); x3 -= bf16_hi(a[nk].z);
+                a[nk].y = pack_bf16(x0, x1);
+                a[nk].w = pack_bf16(x2, x3);
+                lower[nk] = make_uint4(pack_bf16(x0 - bf16_lo(a[nk].y), x1 - bf16_hi(a[nk].y)), 0u, pack_bf16(x2 - bf16_lo(a[nk].w), x3 - bf16_hi(a[nk].w)), 0u);
+                if constexpr (THREE) {      // heads' lanes hold upper and lower terms, the other half middle ones
+                    a[nk] = g < 4 ? make_uint4(a[nk].x, lower[nk].x, a[nk].z, lower[nk].z) : make_uint4(a[nk].y, 0u, a[nk].w, 0u);
                 }
             }
-            // ---- weights
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            top = fmaxf(top, m);
-            const float base = settled(top);
-            float keep = exp2_of(m - base), sum = 0.0f;
+        }
+        // ---- values
+        const unsigned long long keep2 = pair(keep, keep);
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+            if (!PACKED && c > 0 && c * 8 * VE >= width) break;
+            unsigned x[NK][4][4];
 #pragma unroll
             for (int nk = 0; nk < NK; ++nk)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float e = exp2_of(w[nk][i] - base);
-                    sum += e;
-                    if constexpr (!E4M3) w[nk][i] = e;
-                }
-            l = l * keep + sum;
-            m = top;
-            if constexpr (E4M3) {
-                topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 1));
-                topv = fmaxf(topv, __shfl_xor_sync(0xffffffffu, topv, 2));
-                topv = fmaxf(topv, mv);
-                const float basev = settled(topv);
-                keep = exp2_of(mv - basev);
-#pragma unroll
-                for (int nk = 0; nk < NK; ++nk)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[nk][i] = exp2_of(vs[nk][i] - basev + LIFT);
-                mv = topv;
-            }
-            uint4 a[NK], lower[NK];         // left operands of P; bf16: the lowest terms apart
-#pragma unroll
-            for (int nk = 0; nk < NK; ++nk) {
-                float x0 = w[nk][0], x1 = w[nk][1], x2 = w[nk][2], x3 = w[nk][3];
-                if constexpr (E4M3) {
-                    a[nk].x = pack_half(x0, x1);
-                    a[nk].z = pack_half(x2, x3);
-                    const float2 f = unpack_half(a[nk].x), h = unpack_half(a[nk].z);
-                    a[nk].y = pack_half(x0 - f.x, x1 - f.y);
-                    a[nk].w = pack_half(x2 - h.x, x3 - h.y);
-                } else {
-                    a[nk].x = pack_bf16(x0, x1);
-                    a[nk].z = pack_bf16(x2, x3);
-                    x0 -= bf16_lo(a[nk].x); x1 -= bf16_hi(a[nk].x); x2 -= bf16_lo(a[nk].z); x3 -= bf16_hi(a[nk].z);
-                    a[nk].y = pack_bf16(x0, x1);
-                    a[nk].w = pack_bf16(x2, x3);
-                    lower[nk] = make_uint4(pack_bf16(x0 - bf16_lo(a[nk].y), x1 - bf16_hi(a[nk].y)), 0u, pack_bf16(x2 - bf16_lo(a[nk].w), x3 - bf16_hi(a[nk].w)), 0u);
-                    if constexpr (THREE) {      // heads' lanes hold upper and lower terms, the other half middle ones
-                        a[nk] = g < 4 ? make_uint4(a[nk].x, lower[nk].x, a[nk].z, lower[nk].z) : make_uint4(a[nk].y, 0u, a[nk].w, 0u);
+                    const int t = nk * 16 + 8 * (i / 2) + 2 * r + i % 2;
+                    if constexpr (VW == 16) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(values + R::value_at(t, 8 * c + g));
+                        x[nk][i][0] = v.x; x[nk][i][1] = v.y; x[nk][i][2] = v.z; x[nk][i][3] = v.w;
+                    } else {
+                        const uint2 v = *reinterpret_cast<const uint2*>(values + R::value_at(t, 4 * c + g / 2) + g % 2 * 8);
+                        x[nk][i][0] = v.x; x[nk][i][1] = v.y;
                     }
                 }
-            }
-            // ---- values
-            const unsigned long long keep2 = pair(keep, keep);
 #pragma unroll
-            for (int c = 0; c < VC; ++c) {
-                if (!PACKED && c > 0 && c * 8 * VE >= width) break;
-                unsigned x[NK][4][4];
+            for (int i = 0; i < VW / 4; ++i)
 #pragma unroll
-                for (int nk = 0; nk < NK; ++nk)
+                for (int e = 0; e < 2; ++e) {
+                    float y0[4], y1[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int t = nk * 16 + 8 * (i / 2) + 2 * r + i % 2;
-                        if constexpr (VW == 16) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(values + R::value_at(t, 8 * c + g));
-                            x[nk][i][0] = v.x; x[nk][i][1] = v.y; x[nk][i][2] = v.z; x[nk][i][3] = v.w;
-                        } else {
-                            const uint2 v = *reinterpret_cast<const uint2*>(values + R::value_at(t, 4 * c + g / 2) + g % 2 * 8);
-                            x[nk][i][0] = v.x; x[nk][i][1] = v.y;
-                        }
-                    }
-#pragma unroll
-                for (int i = 0; i < VW / 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float y0[4], y1[4];
-#pragma unroll
-                        for (int nk = 0; nk < NK; ++nk) {
-                            if constexpr (E4M3) {
-                                const uint2 b0 = halves_of_e4m3(__byte_perm(x[nk][0][i], x[nk][1][i], e ? 0x7362 : 0x5140));
-                                const uint2 b1 = halves_of_e4m3(__byte_perm(x[nk][2][i], x[nk][3][i], e ? 0x7362 : 0x5140));
-                                if (nk == 0) mma_from_zero<true>(y0, a[nk], b0.x, b1.x);
-                                else mma<true>(y0, a[nk], b0.x, b1.x);
-                                if (nk == 0) mma_from_zero<true>(y1, a[nk], b0.y, b1.y);
-                                else mma<true>(y1, a[nk], b0.y, b1.y);
-                            } else {
-                                const unsigned b0 = __byte_perm(x[nk][0][i], x[nk][1][i], e ? 0x7632 : 0x5410), b1 = __byte_perm(x[nk][2][i], x[nk][3][i], e ? 0x7632 : 0x5410);
-                                if (nk == 0) mma_from_zero<false>(y0, a[nk], b0, b1);
-                                else mma<false>(y0, a[nk], b0, b1);
-                                if constexpr (!THREE) mma<false>(y0, lower[nk], b0, b1);
-                            }
-                        }
+                    for (int nk = 0; nk < NK; ++nk) {
                         if constexpr (E4M3) {
-                            add(c * VE + 4 * i + 2 * e, y0, keep2);
-                            add(c * VE + 4 * i + 2 * e + 1, y1, keep2);
+                            const uint2 b0 = halves_of_e4m3(__byte_perm(x[nk][0][i], x[nk][1][i], e ? 0x7362 : 0x5140));
+                            const uint2 b1 = halves_of_e4m3(__byte_perm(x[nk][2][i], x[nk][3][i], e ? 0x7362 : 0x5140));
+                            if (nk == 0) mma_from_zero<true>(y0, a[nk], b0.x, b1.x);
+                            else mma<true>(y0, a[nk], b0.x, b1.x);
+                            if (nk == 0) mma_from_zero<true>(y1, a[nk], b0.y, b1.y);
+                            else mma<true>(y1, a[nk], b0.y, b1.y);
                         } else {
-                            add(c * VE + 2 * i + e, y0, keep2);
+                            const unsigned b0 = __byte_perm(x[nk][0][i], x[nk][1][i], e ? 0x7632 : 0x5410), b1 = __byte_perm(x[nk][2][i], x[nk][3][i], e ? 0x7632 : 0x5410);
+                            if (nk == 0) mma_from_zero<false>(y0, a[nk], b0, b1);
+                            else mma<false>(y0, a[nk], b0, b1);
+                            if constexpr (!THREE) mma<false>(y0, lower[nk], b0, b1);
                         }
                     }
-            }
+                    if constexpr (E4M3) {
+                        add(c * VE + 4 * i + 2 * e, y0, keep2);
+                        add(c * VE + 4 * i + 2 * e + 1, y1, keep2);
+                    } else {
+                        add(c * VE + 2 * i + e, y0, keep2);
+                    }
+                }
         }
     }
 
@@ -721,92 +720,90 @@ struct FmaWarp {
         const float* q = reinterpret_cast<const float*>(words);
         unsigned long long* weights = reinterpret_cast<unsigned long long*>(words + HT * DP) + warp * (TOKENS * HT + HT);
         unsigned long long* factors = weights + TOKENS * HT;
-        {
-            // ---- scores: every lane of a quad ends with the sums of all heads
-            float sc[TG][HT];
+        // ---- scores: every lane of a quad ends with the sums of all heads
+        float sc[TG][HT];
+#pragma unroll
+        for (int i = 0; i < TG; ++i) {
+            unsigned long long part[HT][2];
+#pragma unroll
+            for (int h = 0; h < HT; ++h) part[h][0] = part[h][1] = 0ull;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                if (!PACKED && c * 16 >= width) break;
+                const ulonglong2 kk = *reinterpret_cast<const ulonglong2*>(keys + R::key_at(g + 8 * i, 4 * c + r));
+#pragma unroll
+                for (int h = 0; h < HT; ++h) {
+                    const ulonglong2 qq = *reinterpret_cast<const ulonglong2*>(q + h * DP + c * 16 + r * 4);
+                    fma2(part[h][0], qq.x, kk.x);
+                    fma2(part[h][1], qq.y, kk.y);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < HT; ++h) {
+                const float2 x = unpair(part[h][0]), y = unpair(part[h][1]);
+                sc[i][h] = (x.x + x.y) + (y.x + y.y);
+                sc[i][h] += __shfl_xor_sync(0xffffffffu, sc[i][h], 1);
+                sc[i][h] += __shfl_xor_sync(0xffffffffu, sc[i][h], 2);
+            }
+        }
+        // ---- weights of heads r, r + 4 over tokens g (and 8 + g)
+        bool moved = false;
+#pragma unroll
+        for (int j = 0; j < OWN; ++j) {
+            const int h = (r + 4 * j) % HT;
+            float w[TG], top = m[j];
 #pragma unroll
             for (int i = 0; i < TG; ++i) {
-                unsigned long long part[HT][2];
+                float x = sc[i][(4 * j) % HT];
 #pragma unroll
-                for (int h = 0; h < HT; ++h) part[h][0] = part[h][1] = 0ull;
-#pragma unroll
-                for (int c = 0; c < KC; ++c) {
-                    if (!PACKED && c * 16 >= width) break;
-                    const ulonglong2 kk = *reinterpret_cast<const ulonglong2*>(keys + R::key_at(g + 8 * i, 4 * c + r));
-#pragma unroll
-                    for (int h = 0; h < HT; ++h) {
-                        const ulonglong2 qq = *reinterpret_cast<const ulonglong2*>(q + h * DP + c * 16 + r * 4);
-                        fma2(part[h][0], qq.x, kk.x);
-                        fma2(part[h][1], qq.y, kk.y);
-                    }
-                }
-#pragma unroll
-                for (int h = 0; h < HT; ++h) {
-                    const float2 x = unpair(part[h][0]), y = unpair(part[h][1]);
-                    sc[i][h] = (x.x + x.y) + (y.x + y.y);
-                    sc[i][h] += __shfl_xor_sync(0xffffffffu, sc[i][h], 1);
-                    sc[i][h] += __shfl_xor_sync(0xffffffffu, sc[i][h], 2);
-                }
+                for (int u = 1; u < 4; ++u) x = r == u ? sc[i][(u + 4 * j) % HT] : x;
+                w[i] = seen >> (g + 8 * i) & 1u ? x * unit : -INFINITY;
+                top = fmaxf(top, w[i]);
             }
-            // ---- weights of heads r, r + 4 over tokens g (and 8 + g)
-            bool moved = false;
 #pragma unroll
-            for (int j = 0; j < OWN; ++j) {
-                const int h = (r + 4 * j) % HT;
-                float w[TG], top = m[j];
+            for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float base = settled(top), keep = exp2_of(m[j] - base);
+            l[j] *= keep;
+            moved |= top != m[j];
+            m[j] = top;
 #pragma unroll
-                for (int i = 0; i < TG; ++i) {
-                    float x = sc[i][(4 * j) % HT];
-#pragma unroll
-                    for (int u = 1; u < 4; ++u) x = r == u ? sc[i][(u + 4 * j) % HT] : x;
-                    w[i] = seen >> (g + 8 * i) & 1u ? x * unit : -INFINITY;
-                    top = fmaxf(top, w[i]);
-                }
-#pragma unroll
-                for (int o = 4; o < 32; o *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                const float base = settled(top), keep = exp2_of(m[j] - base);
-                l[j] *= keep;
-                moved |= top != m[j];
-                m[j] = top;
-#pragma unroll
-                for (int i = 0; i < TG; ++i) {
-                    const float e = exp2_of(w[i] - base);
-                    l[j] += e;
-                    weights[(g + 8 * i) * HT + h] = pair(e, e);
-                }
-                if (g == 0) factors[h] = pair(keep, keep);
+            for (int i = 0; i < TG; ++i) {
+                const float e = exp2_of(w[i] - base);
+                l[j] += e;
+                weights[(g + 8 * i) * HT + h] = pair(e, e);
             }
-            moved = __any_sync(0xffffffffu, moved);
-            __syncwarp();
-            if (moved) {
+            if (g == 0) factors[h] = pair(keep, keep);
+        }
+        moved = __any_sync(0xffffffffu, moved);
+        __syncwarp();
+        if (moved) {
 #pragma unroll
-                for (int h = 0; h < HT; ++h) {
-                    const unsigned long long f = factors[h];
-#pragma unroll
-                    for (int c = 0; c < VC; ++c) {
-                        acc[h][c][0] = mul2(acc[h][c][0], f);
-                        acc[h][c][1] = mul2(acc[h][c][1], f);
-                    }
-                }
-            }
-            // ---- values
-#pragma unroll
-            for (int i = 0; i < VI; ++i) {
-                const int t = i * TPI + which;
-                const unsigned long long* w = weights + t * HT;
+            for (int h = 0; h < HT; ++h) {
+                const unsigned long long f = factors[h];
 #pragma unroll
                 for (int c = 0; c < VC; ++c) {
-                    const ulonglong2 vv = *reinterpret_cast<const ulonglong2*>(values + R::value_at(t, c * 32 + along));
-#pragma unroll
-                    for (int h = 0; h < HT; ++h) {
-                        const unsigned long long x = w[h];
-                        fma2(acc[h][c][0], x, vv.x);
-                        fma2(acc[h][c][1], x, vv.y);
-                    }
+                    acc[h][c][0] = mul2(acc[h][c][0], f);
+                    acc[h][c][1] = mul2(acc[h][c][1], f);
                 }
             }
-            __syncwarp();                  // the weights have been read
         }
+        // ---- values
+#pragma unroll
+        for (int i = 0; i < VI; ++i) {
+            const int t = i * TPI + which;
+            const unsigned long long* w = weights + t * HT;
+#pragma unroll
+            for (int c = 0; c < VC; ++c) {
+                const ulonglong2 vv = *reinterpret_cast<const ulonglong2*>(values + R::value_at(t, c * 32 + along));
+#pragma unroll
+                for (int h = 0; h < HT; ++h) {
+                    const unsigned long long x = w[h];
+                    fma2(acc[h][c][0], x, vv.x);
+                    fma2(acc[h][c][1], x, vv.y);
+                }
+            }
+        }
+        __syncwarp();                  // the weights have been read
     }
 
     __device__ __forceinline__ void finish() {
@@ -940,7 +937,7 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     }
     if (unit >= unit_end) return;
 
-    // ---- its pieces of segments.  Copies run two stages ahead of the arithmetic, into the next pieces as well, so each side
+    // ---- its pieces of segments.  Copies run ahead of the arithmetic, into the next pieces as well, so each side
     // goes through the pieces by itself.
     Walker behind;
     behind.start(unit, unit_end, found_row, found_prefix * tiles_of_heads);
@@ -978,13 +975,13 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
     __syncthreads();
     int at = 0, to = R::STAGES - 1;
     for (;;) {
-        Warp mine_;
-        mine_.begin(p, q_unit);
+        Warp sums_here;
+        sums_here.begin(p, q_unit);
         for (int n = 0; n < piece.tiles; ++n) {
             copies_wait<R::STAGES - 2>();
             __syncwarp();               // this stage has landed for all lanes, and all are done with the one before it
             seen[R::STAGES - 1] = issue_next(to);
-            mine_.step(ring + at * R::STAGE, seen[0], query);
+            sums_here.step(ring + at * R::STAGE, seen[0], query);
 #pragma unroll
             for (int i = 0; i + 1 < R::STAGES; ++i) seen[i] = seen[i + 1];
             at = at + 1 == R::STAGES ? 0 : at + 1;
@@ -994,11 +991,11 @@ __global__ void __launch_bounds__(THREADS, WarpOf<DTYPE, DP, HT, PACKED>::type::
         const bool more = behind.next(range_of, tiles_of_heads, TILE, next);
         const Heads next_heads = heads_of<HEADS>(p, next.head_tile);
         if (more) Warp::load_queries(loaded, p, next.row, next_heads);
-        mine_.finish();
+        sums_here.finish();
         __syncwarp();
         // no copy is under way into the stage read last, which is the next to be filled
         auto sums = [&](int j, int h, int c) { return reinterpret_cast<float*>(rings + j * R::BYTES + to * R::STAGE) + h * DP + c; };
-        mine_.put(sums(warp, 0, 0), ml[warp]);
+        sums_here.put(sums(warp, 0, 0), ml[warp]);
         __syncthreads();
         // ---- the four warps' sums into the result, or into the workspace when the segment is shared with other workers
         const bool whole = piece.begins && piece.ends;
